@@ -383,6 +383,76 @@ int ulm_decode_step(const ulm_decode_layer *layers, int n_layers, const float *x
                     size_t workspace_bytes, int N, int D, int A, int Kc, void *stream);
 
 /* ------------------------------------------------------------------------
+ * The ends of a training, scoring or decoding step.
+ *
+ * ulm_token_logprobs: log probabilities of given tokens under rows of logits
+ * (F.cross_entropy's terms, model.py:160-161), with every row's entropy and its
+ * largest entries. Row r of `rows` starts at element
+ * (r / inner) outer_stride + (r % inner) row_stride of logits and holds V
+ * consecutive elements of `dtype`: any view whose last dimension is dense.
+ *   tokens       (rows,)     the tokens; ignore_index: logprob 0 and no gradient,
+ *                            any other value outside [0, V): logprob NaN
+ *   logprob      (rows,)     out: x_t - ln sum_i e^x_i
+ *   entropy      (rows,)     out: -sum_i p_i ln p_i, masked entries (-inf) counting 0
+ *   top_logprobs (rows, top) out: the `top` largest entries' log probabilities,
+ *   top_tokens   (rows, top) out: and their indices; the lower index first on ties, a NaN
+ *                            above all numbers. top at most ulm_token_logprobs_max_top() and V
+ *   stats        (rows, 2)   out: the row's maximum and ln sum_i e^(x_i - max), for the backward
+ * A row of -inf only has logprob and top_logprobs -inf (0 if ignored), entropy 0, top_tokens
+ * 0, 1, .. and gradient 0. A row with a NaN or +inf has NaN throughout (but for top_tokens and
+ * an ignored token's 0). Workspace of ulm_token_logprobs_workspace_bytes() bytes (may be 0: few
+ * rows are split over several workgroups each and joined in a second launch).
+ *
+ * ulm_token_logprobs_bwd: dlogits (rows, V) dense, in dtype, not aliasing logits, from the same
+ * arguments, the outputs stats, entropy (with dentropy) and top_tokens (with dtop) and the
+ * gradients of logprob (rows,), entropy (rows,) and top_logprobs (rows, top), each fp32 or NULL:
+ *   dx_i = a [i = t] + sum_j c_j [i = top_j] - p_i (a + sum_j c_j + h (ln p_i + entropy)). */
+int ulm_token_logprobs_max_top(void);
+size_t ulm_token_logprobs_workspace_bytes(long long rows, int V, int top);
+int ulm_token_logprobs(const void *logits, int dtype, const long long *tokens, long long rows, long long inner,
+                       long long outer_stride, long long row_stride, int V, int top, long long ignore_index,
+                       float *logprob, float *entropy, float *top_logprobs, long long *top_tokens, float *stats,
+                       void *workspace, size_t workspace_bytes, void *stream);
+int ulm_token_logprobs_bwd(const void *logits, int dtype, const long long *tokens, long long rows, long long inner,
+                           long long outer_stride, long long row_stride, int V, int top, long long ignore_index,
+                           const float *stats, const float *entropy, const long long *top_tokens,
+                           const float *dlogprob, const float *dentropy, const float *dtop, void *dlogits,
+                           void *stream);
+
+/* Embedding lookup (nn.Embedding, model.py:117, 150) and its weight's gradient:
+ * out[n] = scale W[tokens[n]], W (V,D) and out (N,D) dense in dtype; a token
+ * outside [0, V) gives a row of NaN. dweight[v] = scale times the sum of dout[n]
+ * over n with tokens[n] = v, in the order of n (fp32, rounded once), 0 for the
+ * tokens that do not occur; tokens outside [0, V) add to no row. Equal inputs
+ * give equal bits. N at most 2^30. Workspace of ulm_embed_bwd_workspace_bytes() bytes. */
+int ulm_embed_fwd(const void *weight, int dtype, const long long *tokens, long long N, int V, int D, float scale,
+                  void *out, void *stream);
+size_t ulm_embed_bwd_workspace_bytes(long long N, int V, int D);
+int ulm_embed_bwd(const void *dout, int dtype, const long long *tokens, long long N, int V, int D, float scale,
+                  void *dweight, void *workspace, size_t workspace_bytes, void *stream);
+
+/* The global norm of n tensors (a host array of their descriptions) and their
+ * clipping, as the training loop does before the optimizer's step:
+ * norm[0] = sqrt(sum of all squares), summed in double, or the largest |g|;
+ * ulm_clip_grads also writes dst = src min(1, max_norm / (norm + 1e-6)), in
+ * fp32, rounded once. dst may be src (same dtype), and is then left alone when
+ * the factor is 1; otherwise no two regions may overlap. Regions are dense; a NaN among the
+ * elements makes the norm and every result NaN. Workspace of
+ * ulm_grad_norm_workspace_bytes() bytes for the same tensors. */
+typedef struct ulm_grad {
+    const void *src;
+    void *dst;
+    long long numel;
+    int src_dtype, dst_dtype;
+} ulm_grad;
+enum ulm_norm { ULM_NORM_INF = 0, ULM_NORM_2 = 2 };
+size_t ulm_grad_norm_workspace_bytes(const ulm_grad *grads, int n);
+int ulm_grad_norm(const ulm_grad *grads, int n, int norm_type, float *norm, void *workspace, size_t workspace_bytes,
+                  void *stream);
+int ulm_clip_grads(const ulm_grad *grads, int n, int norm_type, float max_norm, float *norm, void *workspace,
+                   size_t workspace_bytes, void *stream);
+
+/* ------------------------------------------------------------------------
  * Diagnostics: HIP-event timing of every chunked-kernel launch (ulm_la and
  * the launches inside ulm_fm_fwd / ulm_fm_bwd) between start and stop, on
  * the stream each launch uses. stop() synchronises on the recorded events

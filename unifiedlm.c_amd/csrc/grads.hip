@@ -1,0 +1,318 @@
+// The global norm of a model's gradients and their clipping to a bound on it
+// (train.py's clip_grad_norm_ before the optimizer's step):
+//
+//     norm = sqrt(sum over all tensors of g^2)  or  max |g|
+//     out  = g min(1, max_norm / (norm + 1e-6))
+//
+// The tensors travel as a table in the kernel's arguments, cut into chunks of equal length
+// that a fixed number of workgroups share; every workgroup leaves one partial norm and the
+// scaling kernel adds those up by itself. Squares are exact in double and summed in it:
+// no gradient of the three types over- or underflows there. Fixed order, no atomics.
+#include <math.h>
+#include <type_traits>
+
+#include "ulm_common.h"
+
+namespace ulm {
+namespace gr {
+
+constexpr int kThreads = 256, kWaves = kThreads / kWave;
+constexpr int kVec = 8, kUnroll = 4;                        // elements a thread takes at once, and how many such
+constexpr int kChunk = kThreads * kVec * kUnroll;           // 8192 elements
+constexpr int kBlocks = 1024;                               // workgroups of a norm launch at most
+constexpr int kTable = 112;                                 // tensors a launch takes: the arguments stay under 4 KB
+constexpr float kEps = 1e-6f;
+
+typedef uint32_t u32x4_any __attribute__((vector_size(16), aligned(2)));   // views start anywhere
+
+struct Table {
+    const char *src[kTable];
+    char *dst[kTable];
+    long long numel[kTable];
+    uint32_t first[kTable + 1];   // the tensors' first chunks, and their number
+    uint8_t src_dt[kTable], dst_dt[kTable];
+    int n;
+};
+
+// the tensor of chunk c
+__device__ __forceinline__ int tensor_of(const Table &t, uint32_t c) {
+    int lo = 0, hi = t.n - 1;
+    while (lo < hi) {
+        const int mid = (lo + hi + 1) / 2;
+        if (t.first[mid] <= c) lo = mid;
+        else hi = mid - 1;
+    }
+    return lo;
+}
+
+template <int DT> __device__ __forceinline__ void load8(const char *p, long long i, float (&x)[kVec]) {
+    if constexpr (DT == ULM_F32) {
+        const u32x4_any a = *reinterpret_cast<const u32x4_any *>(p + 4 * i), b = *reinterpret_cast<const u32x4_any *>(p + 4 * i + 16);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            x[k] = __uint_as_float(a[k]);
+            x[4 + k] = __uint_as_float(b[k]);
+        }
+    } else {
+        const u32x4_any a = *reinterpret_cast<const u32x4_any *>(p + 2 * i);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            if constexpr (DT == ULM_BF16) {
+                x[2 * k] = __uint_as_float(a[k] << 16);
+                x[2 * k + 1] = __uint_as_float(a[k] & 0xffff0000u);
+            } else {
+                x[2 * k] = static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(a[k])));
+                x[2 * k + 1] = static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(a[k] >> 16)));
+            }
+        }
+    }
+}
+
+template <int DT> __device__ __forceinline__ void store8(char *p, long long i, const float (&x)[kVec]) {
+    if constexpr (DT == ULM_F32) {
+        u32x4_any a, b;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            a[k] = __float_as_uint(x[k]);
+            b[k] = __float_as_uint(x[4 + k]);
+        }
+        *reinterpret_cast<u32x4_any *>(p + 4 * i) = a;
+        *reinterpret_cast<u32x4_any *>(p + 4 * i + 16) = b;
+    } else {
+        u32x4_any a;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            if constexpr (DT == ULM_BF16)
+                a[k] = f32_to_bf16_bits(x[2 * k]) | (static_cast<uint32_t>(f32_to_bf16_bits(x[2 * k + 1])) << 16);
+            else
+                a[k] = __builtin_bit_cast(uint16_t, static_cast<_Float16>(x[2 * k])) |
+                       (static_cast<uint32_t>(__builtin_bit_cast(uint16_t, static_cast<_Float16>(x[2 * k + 1]))) << 16);
+        }
+        *reinterpret_cast<u32x4_any *>(p + 2 * i) = a;
+    }
+}
+
+// a chunk's elements of a thread: kUnroll groups of 8, zeros past the tensor's end
+template <int DT>
+__device__ __forceinline__ void load_chunk(const char *p, long long base, long long numel, int tid, float (&x)[kUnroll][kVec]) {
+    if (base + kChunk <= numel) {
+#pragma unroll
+        for (int j = 0; j < kUnroll; ++j) load8<DT>(p, base + (j * kThreads + tid) * kVec, x[j]);
+    } else {
+#pragma unroll
+        for (int j = 0; j < kUnroll; ++j) {
+            const long long i = base + (j * kThreads + tid) * kVec;
+            if (i + kVec <= numel) {
+                load8<DT>(p, i, x[j]);
+            } else {
+#pragma unroll
+                for (int k = 0; k < kVec; ++k) x[j][k] = i + k < numel ? load_as_f32(p, i + k, DT) : 0.f;
+            }
+        }
+    }
+}
+
+// The norms' two measures: an accumulator as a double (the sum of squares) or as the bits
+// of the largest |g| (a NaN's are above infinity's, so it stays).
+template <bool MAX> struct Acc {
+    using T = std::conditional_t<MAX, unsigned long long, double>;
+    static __device__ __forceinline__ T add(T a, T b) {
+        if constexpr (MAX) return a > b ? a : b;
+        else return a + b;
+    }
+    static __device__ __forceinline__ T take(T a, float x) {
+        if constexpr (MAX) {
+            const unsigned long long b = __float_as_uint(x) & 0x7fffffffu;
+            return a > b ? a : b;
+        } else {
+            const double d = x;
+            return __builtin_fma(d, d, a);
+        }
+    }
+    static __device__ __forceinline__ float norm(T a) {
+        if constexpr (MAX) return __uint_as_float(static_cast<uint32_t>(a));
+        else return static_cast<float>(sqrt(a));
+    }
+};
+
+// the workgroup's accumulators joined; every thread gets the result
+template <bool MAX> __device__ typename Acc<MAX>::T join(typename Acc<MAX>::T v) {
+    __shared__ typename Acc<MAX>::T part[kWaves];
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) v = Acc<MAX>::add(v, __shfl_xor(v, off, kWave));
+    if (threadIdx.x % kWave == 0) part[threadIdx.x / kWave] = v;
+    __syncthreads();
+    v = part[0];
+#pragma unroll
+    for (int w = 1; w < kWaves; ++w) v = Acc<MAX>::add(v, part[w]);
+    return v;
+}
+
+template <bool MAX>
+__global__ __launch_bounds__(kThreads) void norm_kernel(Table t, typename Acc<MAX>::T *partial) {
+    typename Acc<MAX>::T acc{};
+    for (uint32_t c = blockIdx.x; c < t.first[t.n]; c += gridDim.x) {
+        const int k = tensor_of(t, c);
+        const long long base = static_cast<long long>(c - t.first[k]) * kChunk;
+        float x[kUnroll][kVec];
+        if (t.src_dt[k] == ULM_F32) load_chunk<ULM_F32>(t.src[k], base, t.numel[k], threadIdx.x, x);
+        else if (t.src_dt[k] == ULM_BF16) load_chunk<ULM_BF16>(t.src[k], base, t.numel[k], threadIdx.x, x);
+        else load_chunk<ULM_F16>(t.src[k], base, t.numel[k], threadIdx.x, x);
+#pragma unroll
+        for (int j = 0; j < kUnroll; ++j)
+#pragma unroll
+            for (int i = 0; i < kVec; ++i) acc = Acc<MAX>::take(acc, x[j][i]);
+    }
+    acc = join<MAX>(acc);
+    if (threadIdx.x == 0) partial[blockIdx.x] = acc;
+}
+
+// the norm of all partials, the same bits in every workgroup
+template <bool MAX> __device__ float total(const typename Acc<MAX>::T *partial, int n) {
+    typename Acc<MAX>::T acc{};
+    for (int i = threadIdx.x; i < n; i += kThreads) acc = Acc<MAX>::add(acc, partial[i]);
+    return Acc<MAX>::norm(join<MAX>(acc));
+}
+
+template <bool MAX>
+__global__ __launch_bounds__(kThreads) void finish_kernel(const typename Acc<MAX>::T *partial, int n, float *norm) {
+    const float v = total<MAX>(partial, n);
+    if (threadIdx.x == 0) *norm = v;
+}
+
+template <int S, int D>
+__device__ __forceinline__ void scale_chunk(const char *src, char *dst, long long base, long long numel, float coef) {
+    const int tid = threadIdx.x;
+    float x[kUnroll][kVec];
+    load_chunk<S>(src, base, numel, tid, x);
+#pragma unroll
+    for (int j = 0; j < kUnroll; ++j) {
+        const long long i = base + (j * kThreads + tid) * kVec;
+#pragma unroll
+        for (int k = 0; k < kVec; ++k) x[j][k] *= coef;
+        if (i + kVec <= numel) {
+            store8<D>(dst, i, x[j]);
+        } else {
+#pragma unroll
+            for (int k = 0; k < kVec; ++k)
+                if (i + k < numel) store_from_f32(dst, i + k, D, x[j][k]);
+        }
+    }
+}
+
+// The chunks scaled, last first: what the norm kernel read last is what the caches still hold.
+template <bool MAX>
+__global__ __launch_bounds__(kThreads) void scale_kernel(Table t, const typename Acc<MAX>::T *partial, int n, float max_norm,
+                                                         float *norm) {
+    const float v = total<MAX>(partial, n);
+    if (norm && blockIdx.x == 0 && threadIdx.x == 0) *norm = v;
+    float coef = max_norm / (v + kEps);
+    if (coef > 1.f) coef = 1.f;   // a NaN stays
+    for (uint32_t b = blockIdx.x; b < t.first[t.n]; b += gridDim.x) {
+        const uint32_t c = t.first[t.n] - 1 - b;
+        const int k = tensor_of(t, c);
+        if (coef == 1.f && t.src[k] == t.dst[k]) continue;   // in place and nothing to change
+        const long long base = static_cast<long long>(c - t.first[k]) * kChunk;
+        const char *src = t.src[k];
+        char *dst = t.dst[k];
+        switch (t.src_dt[k] * 3 + t.dst_dt[k]) {
+#define ULM_GR_CASE(S, D) case S * 3 + D: scale_chunk<S, D>(src, dst, base, t.numel[k], coef); break;
+            ULM_GR_CASE(ULM_F32, ULM_F32) ULM_GR_CASE(ULM_F32, ULM_BF16) ULM_GR_CASE(ULM_F32, ULM_F16)
+            ULM_GR_CASE(ULM_BF16, ULM_F32) ULM_GR_CASE(ULM_BF16, ULM_BF16) ULM_GR_CASE(ULM_BF16, ULM_F16)
+            ULM_GR_CASE(ULM_F16, ULM_F32) ULM_GR_CASE(ULM_F16, ULM_BF16) ULM_GR_CASE(ULM_F16, ULM_F16)
+#undef ULM_GR_CASE
+        }
+    }
+}
+
+static_assert(sizeof(Table) <= 4000, "kernel arguments");
+
+// the tables of up to kTable non-empty tensors each, in order; f(table, chunks)
+template <class F> void tables(const ulm_grad *g, int n, F f) {
+    Table t;
+    t.n = 0;
+    t.first[0] = 0;
+    for (int i = 0; i < n; ++i) {
+        if (g[i].numel <= 0) continue;
+        const long long chunks = (g[i].numel + kChunk - 1) / kChunk;
+        if (t.n == kTable || t.first[t.n] + chunks > UINT32_MAX / 2) {
+            f(t);
+            t.n = 0;
+        }
+        t.src[t.n] = static_cast<const char *>(g[i].src);
+        t.dst[t.n] = static_cast<char *>(g[i].dst);
+        t.numel[t.n] = g[i].numel;
+        t.src_dt[t.n] = static_cast<uint8_t>(g[i].src_dtype);
+        t.dst_dt[t.n] = static_cast<uint8_t>(g[i].dst_dtype);
+        t.first[t.n + 1] = t.first[t.n] + static_cast<uint32_t>(chunks);
+        ++t.n;
+    }
+    if (t.n) f(t);
+}
+
+inline int blocks_of(const Table &t) { return t.first[t.n] < static_cast<uint32_t>(kBlocks) ? static_cast<int>(t.first[t.n]) : kBlocks; }
+
+template <bool MAX>
+int run(const char *fn, const ulm_grad *g, int n, bool scale, float max_norm, float *norm, void *ws, hipStream_t s) {
+    using T = typename Acc<MAX>::T;
+    T *partial = static_cast<T *>(ws);
+    int used = 0;
+    tables(g, n, [&](const Table &t) {
+        const int blocks = blocks_of(t);
+        norm_kernel<MAX><<<dim3(blocks), dim3(kThreads), 0, s>>>(t, partial + used);
+        used += blocks;
+    });
+    if (!scale || used == 0) {
+        finish_kernel<MAX><<<dim3(1), dim3(kThreads), 0, s>>>(partial, used, norm);
+    } else {
+        float *out = norm;
+        tables(g, n, [&](const Table &t) {
+            scale_kernel<MAX><<<dim3(blocks_of(t)), dim3(kThreads), 0, s>>>(t, partial, used, max_norm, out);
+            out = nullptr;
+        });
+    }
+    return check_launch(fn);
+}
+
+int check(const char *fn, const ulm_grad *g, int n, int norm_type, bool scale, float max_norm, const float *norm, const void *ws,
+          size_t bytes) {
+    if (n < 0 || (n > 0 && !g) || !norm || !ws) return fail(ULM_ERR_INVALID, "%s: null pointer or n=%d", fn, n);
+    if (norm_type != ULM_NORM_2 && norm_type != ULM_NORM_INF) return fail(ULM_ERR_INVALID, "%s: bad norm type %d", fn, norm_type);
+    if (scale && !(max_norm >= 0.f)) return fail(ULM_ERR_INVALID, "%s: max_norm must not be negative", fn);
+    for (int i = 0; i < n; ++i) {
+        if (g[i].numel < 0 || g[i].numel > (1LL << 40)) return fail(ULM_ERR_INVALID, "%s: tensor %d has %lld elements", fn, i, g[i].numel);
+        if (!valid_dtype(g[i].src_dtype) || (scale && !valid_dtype(g[i].dst_dtype))) return fail(ULM_ERR_INVALID, "%s: bad dtype of tensor %d", fn, i);
+        if (g[i].numel && (!g[i].src || (scale && !g[i].dst))) return fail(ULM_ERR_INVALID, "%s: null pointer in tensor %d", fn, i);
+        if (scale && g[i].numel && g[i].src == g[i].dst && g[i].src_dtype != g[i].dst_dtype) return fail(ULM_ERR_INVALID, "%s: tensor %d in place in another dtype", fn, i);
+    }
+    const size_t need = ulm_grad_norm_workspace_bytes(g, n);
+    if (bytes < need) return fail(ULM_ERR_INVALID, "%s: workspace %zu < %zu", fn, bytes, need);
+    return ULM_OK;
+}
+
+}  // namespace gr
+}  // namespace ulm
+
+using namespace ulm;
+
+extern "C" size_t ulm_grad_norm_workspace_bytes(const ulm_grad *grads, int n) {
+    size_t blocks = 0;
+    if (grads && n > 0) gr::tables(grads, n, [&](const gr::Table &t) { blocks += gr::blocks_of(t); });
+    return (blocks ? blocks : 1) * sizeof(double);
+}
+
+extern "C" int ulm_grad_norm(const ulm_grad *grads, int n, int norm_type, float *norm, void *workspace, size_t workspace_bytes,
+                             void *stream) {
+    ULM_TRY(gr::check("ulm_grad_norm", grads, n, norm_type, false, 0.f, norm, workspace, workspace_bytes));
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    return norm_type == ULM_NORM_INF ? gr::run<true>("ulm_grad_norm", grads, n, false, 0.f, norm, workspace, s)
+                                     : gr::run<false>("ulm_grad_norm", grads, n, false, 0.f, norm, workspace, s);
+}
+
+extern "C" int ulm_clip_grads(const ulm_grad *grads, int n, int norm_type, float max_norm, float *norm, void *workspace,
+                              size_t workspace_bytes, void *stream) {
+    ULM_TRY(gr::check("ulm_clip_grads", grads, n, norm_type, true, max_norm, norm, workspace, workspace_bytes));
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    return norm_type == ULM_NORM_INF ? gr::run<true>("ulm_clip_grads", grads, n, true, max_norm, norm, workspace, s)
+                                     : gr::run<false>("ulm_clip_grads", grads, n, true, max_norm, norm, workspace, s);
+}

@@ -1,0 +1,517 @@
+// Log probabilities of given tokens, with each row's entropy and its largest
+// entries, and the logits' gradient: the classifier's end of a training step
+// (F.cross_entropy over the logits, model.py:160-161), of scoring and of a
+// decode position.
+//
+// For a row x of V logits, m = max x, d_i = x_i - m, s = sum e^d_i:
+//
+//     logprob = d_t - ln s      entropy = ln s - (sum e^d_i d_i) / s      p_i = e^d_i / s
+//     dx_i    = a [i = t] + sum_j c_j [i = top_j] - p_i (G + h (ln p_i + H)),  G = a + sum_j c_j
+//
+// with a, h, c_j the gradients of logprob, entropy and the top log probabilities.
+#include <type_traits>
+
+#include "ulm_common.h"
+
+namespace ulm {
+namespace lp {
+
+constexpr int kThreads = 256;
+constexpr int kUnroll = 4;            // 16-byte loads in flight per thread
+constexpr int kMaxTop = 64;           // one lane of a wave each
+constexpr int kMaxParts = 16;
+constexpr int kCap = 1024;            // candidates held at once
+constexpr float kLog2e = 1.44269504088896341f;
+constexpr float kFloor = -1e4f;       // e^d is 0 from here on: keeps 0 x (-inf) out of the sums
+
+typedef uint32_t u32x4_any __attribute__((vector_size(16), aligned(2)));   // rows may start anywhere
+
+template <int DT> struct Elem { static constexpr int vec = DT == ULM_F32 ? 4 : 8, bytes = DT == ULM_F32 ? 4 : 2; };
+
+template <int DT> __device__ __forceinline__ void unpack(const u32x4_any &w, float (&x)[Elem<DT>::vec]) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        if constexpr (DT == ULM_F32) {
+            x[k] = __uint_as_float(w[k]);
+        } else if constexpr (DT == ULM_BF16) {
+            x[2 * k] = __uint_as_float(w[k] << 16);
+            x[2 * k + 1] = __uint_as_float(w[k] & 0xffff0000u);
+        } else {
+            x[2 * k] = static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(w[k])));
+            x[2 * k + 1] = static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(w[k] >> 16)));
+        }
+    }
+}
+
+template <int DT> __device__ __forceinline__ uint32_t pack_word(float a, float b) {
+    if constexpr (DT == ULM_BF16) {
+        return f32_to_bf16_bits(a) | (static_cast<uint32_t>(f32_to_bf16_bits(b)) << 16);
+    } else {
+        return __builtin_bit_cast(uint16_t, static_cast<_Float16>(a)) |
+               (static_cast<uint32_t>(__builtin_bit_cast(uint16_t, static_cast<_Float16>(b))) << 16);
+    }
+}
+
+// x's elements [i, i + vec) of a row that ends at `end`, -inf past it
+template <int DT>
+__device__ __forceinline__ void load_vec(const char *row, int i, int end, float (&x)[Elem<DT>::vec]) {
+    constexpr int V = Elem<DT>::vec;
+    if (i + V <= end) {
+        unpack<DT>(*reinterpret_cast<const u32x4_any *>(row + static_cast<size_t>(i) * Elem<DT>::bytes), x);
+    } else {
+#pragma unroll
+        for (int k = 0; k < V; ++k) x[k] = i + k < end ? load_as_f32(row, i + k, DT) : -INFINITY;
+    }
+}
+
+// Unique keys in the order of the alternatives: by value (a NaN above all), then by the lower index.
+__device__ __forceinline__ uint64_t key_of(float x, int i) {
+    uint32_t b = __float_as_uint(x + 0.f);   // -0 and 0 are one value
+    b = x != x ? 0xffffffffu : (b & 0x80000000u) ? ~b : b | 0x80000000u;
+    return static_cast<uint64_t>(b) << 32 | (0xffffffffu - static_cast<uint32_t>(i));
+}
+__device__ __forceinline__ int index_of(uint64_t key) { return static_cast<int>(0xffffffffu - static_cast<uint32_t>(key)); }
+__device__ __forceinline__ float value_of(uint64_t key) {
+    const uint32_t b = key >> 32;
+    return __uint_as_float((b & 0x80000000u) ? b & 0x7fffffffu : ~b);
+}
+
+__device__ __forceinline__ float exp_of(float d) { return __builtin_amdgcn_exp2f(d * kLog2e); }
+
+// The sums of a set of logits about their maximum m: s = sum e^(x - m), u = sum e^(x - m) (x - m).
+struct Sums {
+    float m, s, u;
+    __device__ __forceinline__ void rebase(float to) {   // to >= m
+        const float d = m == to ? 0.f : fmaxf(m - to, kFloor), f = exp_of(d);
+        u = f * __builtin_fmaf(s, d, u);
+        s *= f;
+        m = to;
+    }
+    __device__ __forceinline__ void add(Sums o) {
+        const float to = fmaxf(m, o.m);
+        rebase(to);
+        o.rebase(to);
+        s += o.s;
+        u += o.u;
+    }
+};
+
+__device__ __forceinline__ Sums wave_add(Sums v) {
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) {
+        Sums o;
+        o.m = __shfl_xor(v.m, off, kWave);
+        o.s = __shfl_xor(v.s, off, kWave);
+        o.u = __shfl_xor(v.u, off, kWave);
+        // the same operations in the same order on both lanes: both end with the same bits
+        if (threadIdx.x & off) {
+            o.add(v);
+            v = o;
+        } else {
+            v.add(o);
+        }
+    }
+    return v;
+}
+
+// Workgroup b of n: the grid's second dimension takes what the first cannot count.
+constexpr long long kGridX = 1 << 20;
+inline dim3 grid_of(long long n) {
+    return n <= kGridX ? dim3(static_cast<unsigned>(n)) : dim3(kGridX, static_cast<unsigned>((n + kGridX - 1) / kGridX));
+}
+__device__ __forceinline__ long long block_id() { return static_cast<long long>(blockIdx.y) * gridDim.x + blockIdx.x; }
+
+struct Rows {
+    const char *x;
+    const long long *tokens;
+    long long inner, outer_stride, row_stride;   // row r starts at (r / inner) outer_stride + (r % inner) row_stride elements
+    long long ignore, rows;
+    int V, top, parts, part_len;
+    __device__ __forceinline__ const char *row(long long r, int bytes) const {
+        return x + ((r / inner) * outer_stride + (r % inner) * row_stride) * bytes;
+    }
+};
+
+struct Outs {
+    float *logprob, *entropy, *top_logprobs, *stats;
+    long long *top_tokens;
+};
+
+// what every row ends with, on one thread: its log probability, entropy and (m, ln s)
+template <int DT>
+__device__ __forceinline__ void finish_row(const Rows &a, const Outs &o, long long r, Sums v, float &m, float &logs) {
+    logs = v.s > 0.f ? logf(v.s) : v.s == 0.f ? -INFINITY : v.s;   // an empty row: -inf; a NaN stays
+    m = v.m;
+    const long long t = a.tokens[r];
+    float lp = 0.f;
+    if (t != a.ignore) {
+        lp = __uint_as_float(0x7fc00000u);
+        if (t >= 0 && t < a.V) {
+            const float x = load_as_f32(a.row(r, Elem<DT>::bytes), t, DT);
+            lp = v.s == 0.f ? -INFINITY : (x - m) - logs;
+        }
+    }
+    o.logprob[r] = lp;
+    o.entropy[r] = v.s == 0.f ? 0.f : logs - v.u / v.s;
+    o.stats[2 * r] = m;
+    o.stats[2 * r + 1] = logs;
+}
+
+__device__ __forceinline__ void put_top(const Rows &a, const Outs &o, long long r, int rank, uint64_t key, float m, float logs) {
+    const float x = value_of(key);
+    o.top_logprobs[r * a.top + rank] = logs == -INFINITY ? -INFINITY : (x - m) - logs;
+    o.top_tokens[r * a.top + rank] = index_of(key);
+}
+
+// The `top` largest of elements [e0, e1), as keys in `list`, and how many of the list's
+// entries there are (at least `top` where there are as many elements).
+//
+// Every thread knows its own largest element; the top-th largest of 64 groups' maxima is
+// no more than the top-th largest element of all, and whatever is no less than it lies in
+// the at most `top` groups whose maximum is. Those threads read their elements again.
+// Should more than kCap elements pass, the top-th largest of the kCap that were kept is a
+// higher such bound, and all but `top` of those kCap fall below it: every turn leaves out
+// kCap - top elements or more.
+template <int DT>
+__device__ int candidates(const char *row, int e0, int e1, int top, uint64_t mine, bool all, uint64_t *list,
+                          uint64_t *groups, int *count, uint64_t *bound) {
+    constexpr int V = Elem<DT>::vec;
+    const int tid = threadIdx.x, lane = tid % kWave;
+    groups[tid] = mine;
+    if (tid == 0) *count = 0;
+    __syncthreads();
+    if (tid < kWave) {
+        uint64_t k = groups[lane];
+#pragma unroll
+        for (int w = 1; w < kThreads / kWave; ++w) {
+            const uint64_t o = groups[lane + w * kWave];
+            k = o > k ? o : k;
+        }
+        int rank = 0;
+        for (int j = 0; j < kWave; ++j) {
+            const uint64_t o = __shfl(k, j, kWave);
+            rank += o > k || (o == k && j < lane);   // empty groups share the key 0
+        }
+        if (rank == top - 1) *bound = k;
+    }
+    __syncthreads();
+    for (;;) {
+        const uint64_t low = *bound;
+        if (all || mine >= low) {
+            for (int i = e0 + tid * V; i < e1; i += kThreads * V) {
+                float x[V];
+                load_vec<DT>(row, i, e1, x);
+#pragma unroll
+                for (int k = 0; k < V; ++k) {
+                    const uint64_t key = key_of(x[k], i + k);
+                    if (i + k < e1 && key >= low) {
+                        const int at = atomicAdd(count, 1);
+                        if (at < kCap) list[at] = key;
+                    }
+                }
+            }
+        }
+        __syncthreads();
+        const int n = *count;
+        if (n <= kCap) return n;
+        __syncthreads();
+        if (tid == 0) *count = 0;
+        for (int i = tid; i < kCap; i += kThreads) {
+            const uint64_t k = list[i];
+            int rank = 0;
+            for (int j = 0; j < kCap; ++j) rank += list[j] > k;
+            if (rank == top - 1) *bound = k;
+        }
+        __syncthreads();
+    }
+}
+
+// One workgroup per (row, part). With one part it writes the row's outputs, with more the
+// part's sums and its `top` best keys in order (0 where it has fewer).
+template <int DT, bool TOP>
+__global__ __launch_bounds__(kThreads) void fwd_kernel(Rows a, Outs o, Sums *part_sums, uint64_t *part_keys) {
+    constexpr int V = Elem<DT>::vec, kTile = kThreads * V * kUnroll;
+    const long long id = block_id(), r = id / a.parts;
+    if (r >= a.rows) return;
+    const int tid = threadIdx.x, part = static_cast<int>(id % a.parts);
+    const char *row = a.row(r, Elem<DT>::bytes);
+    const int e0 = part * a.part_len, e1 = min(a.V, e0 + a.part_len);
+
+    Sums v{-INFINITY, 0.f, 0.f};
+    float best = -INFINITY;
+    int best_at = e0;   // the tile that holds the thread's first largest element
+    for (int t = e0; t < e1; t += kTile) {
+        float x[kUnroll][V];
+        if (t + kTile <= e1) {
+            u32x4_any w[kUnroll];
+#pragma unroll
+            for (int j = 0; j < kUnroll; ++j)
+                w[j] = *reinterpret_cast<const u32x4_any *>(row + static_cast<size_t>(t + (j * kThreads + tid) * V) * Elem<DT>::bytes);
+#pragma unroll
+            for (int j = 0; j < kUnroll; ++j) unpack<DT>(w[j], x[j]);
+        } else {
+#pragma unroll
+            for (int j = 0; j < kUnroll; ++j) load_vec<DT>(row, t + (j * kThreads + tid) * V, e1, x[j]);
+        }
+        float most = x[0][0];
+#pragma unroll
+        for (int j = 0; j < kUnroll; ++j)
+#pragma unroll
+            for (int k = 0; k < V; ++k) most = fmaxf(most, x[j][k]);
+        if (TOP && most > best) {
+            best = most;
+            best_at = t;
+        }
+        if (most > v.m) v.rebase(most);
+        if (v.m == -INFINITY) {   // nothing but masked elements so far (or NaN)
+#pragma unroll
+            for (int j = 0; j < kUnroll; ++j)
+#pragma unroll
+                for (int k = 0; k < V; ++k) v.s += x[j][k] != x[j][k] ? x[j][k] : 0.f;
+            continue;
+        }
+#pragma unroll
+        for (int j = 0; j < kUnroll; ++j)
+#pragma unroll
+            for (int k = 0; k < V; ++k) {
+                const float d = x[j][k] - v.m, e = exp_of(d);
+                v.s += e;
+                v.u = __builtin_fmaf(e, fmaxf(d, kFloor), v.u);
+            }
+    }
+
+    __shared__ Sums waves[kThreads / kWave];
+    const bool odd = v.s != v.s;   // a NaN among the thread's elements
+    const Sums w = wave_add(v);
+    if (tid % kWave == 0) waves[tid / kWave] = w;
+    __syncthreads();
+    Sums all = waves[0];
+#pragma unroll
+    for (int k = 1; k < kThreads / kWave; ++k) all.add(waves[k]);
+
+    float m = 0.f, logs = 0.f;
+    __shared__ float ml[2];
+    if (tid == 0) {
+        if (a.parts == 1) {
+            finish_row<DT>(a, o, r, all, m, logs);
+            ml[0] = m;
+            ml[1] = logs;
+        } else {
+            part_sums[id] = all;
+        }
+    }
+    if constexpr (TOP) {
+        __shared__ uint64_t list[kCap], groups[kThreads], bound;
+        __shared__ int count;
+        uint64_t mine = 0;   // the key of the thread's largest element that is no NaN
+        for (int j = kUnroll - 1; j >= 0; --j) {
+            const int i = best_at + (j * kThreads + tid) * V;
+            if (i >= e1) continue;
+            float x[V];
+            load_vec<DT>(row, i, e1, x);
+#pragma unroll
+            for (int k = V - 1; k >= 0; --k)
+                if (i + k < e1 && x[k] == best) mine = key_of(x[k], i + k);
+        }
+        const int n = candidates<DT>(row, e0, e1, a.top, mine, odd, list, groups, &count, &bound);
+        m = ml[0];
+        logs = ml[1];
+        for (int i = tid; i < n; i += kThreads) {
+            const uint64_t k = list[i];
+            int rank = 0;
+            for (int j = 0; j < n; ++j) rank += list[j] > k;
+            if (rank >= a.top) continue;
+            if (a.parts == 1) put_top(a, o, r, rank, k, m, logs);
+            else part_keys[id * a.top + rank] = k;
+        }
+        if (a.parts > 1)
+            for (int i = n + tid; i < a.top; i += kThreads) part_keys[id * a.top + i] = 0;
+    }
+}
+
+// The parts of a row joined: one workgroup per row.
+template <int DT, bool TOP>
+__global__ __launch_bounds__(kThreads) void join_kernel(Rows a, Outs o, const Sums *part_sums, const uint64_t *part_keys) {
+    const long long r = blockIdx.x;
+    const int tid = threadIdx.x;
+    __shared__ float ml[2];
+    __shared__ uint64_t list[kMaxParts * kMaxTop];
+    const int n = TOP ? a.parts * a.top : 0;
+    for (int i = tid; i < n; i += kThreads) list[i] = part_keys[r * n + i];
+    if (tid == 0) {
+        Sums all = part_sums[r * a.parts];
+        for (int p = 1; p < a.parts; ++p) all.add(part_sums[r * a.parts + p]);
+        finish_row<DT>(a, o, r, all, ml[0], ml[1]);
+    }
+    if constexpr (TOP) {
+        __syncthreads();
+        const float m = ml[0], logs = ml[1];
+        for (int i = tid; i < n; i += kThreads) {
+            const uint64_t k = list[i];
+            if (k == 0) continue;
+            int rank = 0;
+            for (int j = 0; j < n; ++j) rank += list[j] > k;
+            if (rank < a.top) put_top(a, o, r, rank, k, m, logs);
+        }
+    }
+}
+
+struct Grads {
+    const float *stats, *entropy, *dlogprob, *dentropy, *dtop;
+    const long long *top_tokens;
+    char *dx;   // (rows, V), dense
+};
+
+// One workgroup per (row, tile of elements).
+template <int DT, bool ENT>
+__global__ __launch_bounds__(kThreads) void bwd_kernel(Rows a, Grads g, int tiles) {
+    constexpr int V = Elem<DT>::vec, kTile = kThreads * V * kUnroll, B = Elem<DT>::bytes;
+    const long long id = block_id(), r = id / tiles;
+    if (r >= a.rows) return;
+    const int tid = threadIdx.x, e0 = static_cast<int>(id % tiles) * kTile, e1 = min(a.V, e0 + kTile);
+    const char *row = a.row(r, B);
+    char *out = g.dx + static_cast<size_t>(r) * a.V * B;
+
+    const float m = g.stats[2 * r], logs = g.stats[2 * r + 1];
+    const float h = ENT ? g.dentropy[r] : 0.f, H = ENT ? g.entropy[r] : 0.f;
+    const long long t = a.tokens[r];
+    float da = g.dlogprob && t != a.ignore ? g.dlogprob[r] : 0.f;
+    if (t != a.ignore && (t < 0 || t >= a.V)) da = __uint_as_float(0x7fc00000u);
+    float G = da;
+    if (g.dtop)
+        for (int j = 0; j < a.top; ++j) G += g.dtop[r * a.top + j];
+    const bool empty = m == -INFINITY && logs == -INFINITY;
+    auto grad = [&](float x) {   // without the tokens' own terms
+        const float d = x - m, p = exp_of(d - logs);
+        const float f = ENT ? __builtin_fmaf(h, (fmaxf(d, kFloor) - logs) + H, G) : G;
+        return empty ? 0.f : -p * f;
+    };
+#pragma unroll
+    for (int j = 0; j < kUnroll; ++j) {
+        const int i = e0 + (j * kThreads + tid) * V;
+        if (i >= e1) continue;
+        float x[V];
+        load_vec<DT>(row, i, e1, x);
+        const long long own = t - i;   // the token's place among these
+#pragma unroll
+        for (int k = 0; k < V; ++k) {
+            x[k] = grad(x[k]);
+            if (own == k && !empty) x[k] += da;
+        }
+        if (i + V <= e1) {
+            u32x4_any w;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                if constexpr (DT == ULM_F32) w[k] = __float_as_uint(x[k]);
+                else w[k] = pack_word<DT>(x[2 * k], x[2 * k + 1]);
+            }
+            *reinterpret_cast<u32x4_any *>(out + static_cast<size_t>(i) * B) = w;
+        } else {
+#pragma unroll
+            for (int k = 0; k < V; ++k)
+                if (i + k < e1) store_from_f32(out, i + k, DT, x[k]);
+        }
+    }
+    if (!g.dtop || empty) return;
+    __syncthreads();   // the alternatives' elements are written again, with their own terms
+    if (tid < a.top) {
+        const long long i = g.top_tokens[r * a.top + tid];
+        if (i >= e0 && i < e1)
+            store_from_f32(out, i, DT, grad(load_as_f32(row, i, DT)) + g.dtop[r * a.top + tid] + (i == t ? da : 0.f));
+    }
+}
+
+// Parts a row is split into: a function of the sizes, the same for the workspace and the launch.
+inline int parts_of(long long rows, int V) {
+    if (rows >= 512) return 1;
+    long long p = (1024 + rows - 1) / rows;
+    const long long most = (V + 2047) / 2048;
+    if (p > most) p = most;
+    if (p > kMaxParts) p = kMaxParts;
+    return p < 1 ? 1 : static_cast<int>(p);
+}
+
+}  // namespace lp
+}  // namespace ulm
+
+using namespace ulm;
+
+static int check_rows(const char *fn, long long rows, long long inner, int V, int top, int dtype) {
+    if (rows < 1 || rows > (1LL << 34) || inner < 1 || V < 1 || V > (1 << 30))
+        return fail(ULM_ERR_INVALID, "%s: bad sizes rows=%lld inner=%lld V=%d", fn, rows, inner, V);
+    if (top < 0 || top > lp::kMaxTop || top > V) return fail(ULM_ERR_INVALID, "%s: top=%d outside 0 .. min(V, %d)", fn, top, lp::kMaxTop);
+    if (!valid_dtype(dtype)) return fail(ULM_ERR_INVALID, "%s: bad dtype %d", fn, dtype);
+    return ULM_OK;
+}
+
+extern "C" int ulm_token_logprobs_max_top(void) { return lp::kMaxTop; }
+
+extern "C" size_t ulm_token_logprobs_workspace_bytes(long long rows, int V, int top) {
+    if (rows < 1 || V < 1 || top < 0 || top > lp::kMaxTop) return 0;
+    const int parts = lp::parts_of(rows, V);
+    if (parts == 1) return 0;
+    Carver c(nullptr);
+    c.take<lp::Sums>(static_cast<size_t>(rows) * parts);
+    c.take<uint64_t>(static_cast<size_t>(rows) * parts * top);
+    return c.off;
+}
+
+extern "C" int ulm_token_logprobs(const void *logits, int dtype, const long long *tokens, long long rows, long long inner,
+                                  long long outer_stride, long long row_stride, int V, int top, long long ignore_index,
+                                  float *logprob, float *entropy, float *top_logprobs, long long *top_tokens, float *stats,
+                                  void *workspace, size_t workspace_bytes, void *stream) {
+    ULM_TRY(check_rows("ulm_token_logprobs", rows, inner, V, top, dtype));
+    ULM_REQUIRE(logits && tokens && logprob && entropy && stats && (top == 0 || (top_logprobs && top_tokens)),
+                "ulm_token_logprobs: null pointer");
+    const int parts = lp::parts_of(rows, V);
+    const size_t need = ulm_token_logprobs_workspace_bytes(rows, V, top);
+    ULM_REQUIRE(workspace_bytes >= need && (need == 0 || workspace), "ulm_token_logprobs: workspace %zu < %zu", workspace_bytes, need);
+    Carver c(workspace);
+    lp::Sums *sums = parts > 1 ? c.take<lp::Sums>(static_cast<size_t>(rows) * parts) : nullptr;
+    uint64_t *keys = parts > 1 ? c.take<uint64_t>(static_cast<size_t>(rows) * parts * top) : nullptr;
+    // parts of whole 8-element vectors
+    const int part_len = parts == 1 ? V : (V + parts * 8 - 1) / (parts * 8) * 8;
+    const lp::Rows a{static_cast<const char *>(logits), tokens, inner, outer_stride, row_stride, ignore_index, rows, V, top, parts, part_len};
+    const lp::Outs o{logprob, entropy, top_logprobs, stats, top_tokens};
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    auto launch = [&](auto dt, auto with_top) {
+        constexpr int DT = decltype(dt)::value;
+        constexpr bool TOP = decltype(with_top)::value;
+        lp::fwd_kernel<DT, TOP><<<lp::grid_of(rows * parts), dim3(lp::kThreads), 0, s>>>(a, o, sums, keys);
+        if (parts > 1)
+            lp::join_kernel<DT, TOP><<<lp::grid_of(rows), dim3(lp::kThreads), 0, s>>>(a, o, sums, keys);
+    };
+    auto by_top = [&](auto dt) {
+        if (top) launch(dt, std::true_type{});
+        else launch(dt, std::false_type{});
+    };
+    if (dtype == ULM_F32) by_top(std::integral_constant<int, ULM_F32>{});
+    else if (dtype == ULM_BF16) by_top(std::integral_constant<int, ULM_BF16>{});
+    else by_top(std::integral_constant<int, ULM_F16>{});
+    return check_launch("ulm_token_logprobs");
+}
+
+extern "C" int ulm_token_logprobs_bwd(const void *logits, int dtype, const long long *tokens, long long rows, long long inner,
+                                      long long outer_stride, long long row_stride, int V, int top, long long ignore_index,
+                                      const float *stats, const float *entropy, const long long *top_tokens,
+                                      const float *dlogprob, const float *dentropy, const float *dtop, void *dlogits,
+                                      void *stream) {
+    ULM_TRY(check_rows("ulm_token_logprobs_bwd", rows, inner, V, top, dtype));
+    ULM_REQUIRE(logits && tokens && stats && dlogits && (!dentropy || entropy) && (!dtop || (top_tokens && top)),
+                "ulm_token_logprobs_bwd: null pointer");
+    ULM_REQUIRE(dlogits != logits, "ulm_token_logprobs_bwd: dlogits must not alias logits");
+    const int tile = lp::kThreads * lp::kUnroll * (dtype == ULM_F32 ? 4 : 8), tiles = (V + tile - 1) / tile;
+    const lp::Rows a{static_cast<const char *>(logits), tokens, inner, outer_stride, row_stride, ignore_index, rows, V, top, 1, V};
+    const lp::Grads g{stats, entropy, dlogprob, dentropy, dtop, top_tokens, static_cast<char *>(dlogits)};
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    const dim3 grid = lp::grid_of(rows * tiles), block(lp::kThreads);
+    auto launch = [&](auto dt) {
+        constexpr int DT = decltype(dt)::value;
+        if (dentropy) lp::bwd_kernel<DT, true><<<grid, block, 0, s>>>(a, g, tiles);
+        else lp::bwd_kernel<DT, false><<<grid, block, 0, s>>>(a, g, tiles);
+    };
+    if (dtype == ULM_F32) launch(std::integral_constant<int, ULM_F32>{});
+    else if (dtype == ULM_BF16) launch(std::integral_constant<int, ULM_BF16>{});
+    else launch(std::integral_constant<int, ULM_F16>{});
+    return check_launch("ulm_token_logprobs_bwd");
+}

@@ -13,9 +13,13 @@ Matmul operands are bf16 with fp32 accumulation and an fp32 chunk state kept
 on chip; c, q and all their gradients are fp32, as in the reference.
 
 Besides the operator this module exposes the relu^2 slot address
-(model.py:70-72) as an autograd Function and the three per-token decode
-kernels used by UnifiedBlock.step.
+(model.py:70-72) as an autograd Function, the three per-token decode
+kernels used by UnifiedBlock.step, and the two ends of a step: the embedding
+lookup, the log probabilities of given tokens (the loss), and the gradients'
+norm and clipping.
 """
+import math
+from collections import namedtuple
 from typing import Optional
 
 import torch
@@ -789,3 +793,368 @@ def decode_deferred(S, pv, pr, m, flush, q, g, x, ymu, cj=None):
         call("ulm_decode_read", ptr(_f32c(S)), ptr(_f32c(pv)), ptr(_f32c(cj)), m, ptr(_f32c(q)), ptr(_f32c(g)),
              ptr(_f32c(x)), ptr(_f32c(ymu)), ptr(out), N, D, A, st)
     return out
+
+
+# ---------------------------------------------------------------------------
+# log probabilities of given tokens (F.cross_entropy over the logits,
+# model.py:160-161), with each row's entropy and its largest entries
+
+TokenLogprobs = namedtuple("TokenLogprobs", "logprob entropy top_logprobs top_tokens")
+
+
+def _int_tokens(tokens):
+    """Token ids as the kernels read them."""
+    return tokens.to(torch.int64).contiguous()
+
+
+def _rows(logits):
+    """(tensor, inner, outer stride, row stride): the rows of (..., V) logits as
+    the kernels address them, without a copy where the last dimension is dense
+    and the leading ones collapse into two."""
+    dims = [[n, st] for n, st in zip(logits.shape[:-1], logits.stride()[:-1]) if n != 1]
+    groups = []
+    for n, st in dims:
+        if groups and groups[-1][1] == n * st:
+            groups[-1] = [groups[-1][0] * n, st]
+        else:
+            groups.append([n, st])
+    V = logits.shape[-1]
+    if len(groups) > 2 or (V > 1 and logits.stride(-1) != 1):
+        return logits.contiguous(), max(1, logits.numel() // V), 0, V
+    if len(groups) == 2:
+        return logits, groups[1][0], groups[0][1], groups[1][1]
+    return (logits, groups[0][0], 0, groups[0][1]) if groups else (logits, 1, 0, V)
+
+
+@torch.library.custom_op("ulm::token_logprobs", mutates_args=())
+def token_logprobs_fwd(logits: Tensor, tokens: Tensor, top: int,
+                       ignore_index: int) -> tuple[Tensor, Tensor, Tensor, Tensor, Tensor]:
+    """(logprob, entropy, top_logprobs, top_tokens, stats (..., 2)): ulm_token_logprobs."""
+    lead, V = logits.shape[:-1], logits.shape[-1]
+    f32 = dict(device=logits.device, dtype=torch.float32)
+    logprob, entropy = torch.empty(lead, **f32), torch.empty(lead, **f32)
+    top_logprobs = torch.empty(*lead, top, **f32)
+    top_tokens = torch.empty(*lead, top, device=logits.device, dtype=torch.int64)
+    stats = torch.empty(*lead, 2, **f32)
+    rows = logprob.numel()
+    if rows:
+        with torch.cuda.device(logits.device):
+            x, inner, outer_stride, row_stride = _rows(logits)
+            tok = _int_tokens(tokens)
+            ws_bytes = nat.lib().ulm_token_logprobs_workspace_bytes(rows, V, top)
+            ws = torch.empty(max(ws_bytes, 1), device=logits.device, dtype=torch.uint8)
+            call("ulm_token_logprobs", ptr(x), nat.dtype_code(logits.dtype), ptr(tok), rows, inner, outer_stride,
+                 row_stride, V, top, ignore_index, ptr(logprob), ptr(entropy), ptr(top_logprobs), ptr(top_tokens),
+                 ptr(stats), ptr(ws), ws_bytes, nat.stream_of(logits))
+    return logprob, entropy, top_logprobs, top_tokens, stats
+
+
+@token_logprobs_fwd.register_fake
+def _token_logprobs_fake(logits, tokens, top, ignore_index):
+    lead = logits.shape[:-1]
+    e = lambda *shape, dtype=torch.float32: logits.new_empty(*shape, dtype=dtype)  # noqa: E731
+    return e(lead), e(lead), e((*lead, top)), e((*lead, top), dtype=torch.int64), e((*lead, 2))
+
+
+@torch.library.custom_op("ulm::token_logprobs_bwd", mutates_args=())
+def token_logprobs_bwd(logits: Tensor, tokens: Tensor, top: int, ignore_index: int, stats: Tensor, entropy: Tensor,
+                       top_tokens: Tensor, dlogprob: Optional[Tensor], dentropy: Optional[Tensor],
+                       dtop: Optional[Tensor]) -> Tensor:
+    """The logits' gradient in their dtype, dense: ulm_token_logprobs_bwd."""
+    V = logits.shape[-1]
+    out = torch.empty(logits.shape, device=logits.device, dtype=logits.dtype)
+    rows = out.numel() // V
+    if rows:
+        with torch.cuda.device(logits.device):
+            x, inner, outer_stride, row_stride = _rows(logits)
+            tok = _int_tokens(tokens)
+            up = [None if t is None or t.numel() == 0 else t.float().contiguous() for t in (dlogprob, dentropy, dtop)]
+            call("ulm_token_logprobs_bwd", ptr(x), nat.dtype_code(logits.dtype), ptr(tok), rows, inner, outer_stride,
+                 row_stride, V, top, ignore_index, ptr(stats.contiguous()), ptr(entropy.contiguous()),
+                 ptr(top_tokens.contiguous()), *map(ptr, up), ptr(out), nat.stream_of(logits))
+    return out
+
+
+@token_logprobs_bwd.register_fake
+def _token_logprobs_bwd_fake(logits, tokens, top, ignore_index, stats, entropy, top_tokens, dlogprob, dentropy, dtop):
+    return torch.empty_like(logits, memory_format=torch.contiguous_format)
+
+
+def _token_logprobs_setup(ctx, inputs, output):
+    logits, tokens, ctx.top, ctx.ignore_index = inputs
+    _, entropy, _, top_tokens, stats = output
+    ctx.save_for_backward(logits, tokens, stats, entropy, top_tokens)
+    ctx.mark_non_differentiable(top_tokens, stats)
+    ctx.set_materialize_grads(False)
+
+
+def _token_logprobs_backward(ctx, dlogprob, dentropy, dtop, _dtokens, _dstats):
+    if dlogprob is None and dentropy is None and dtop is None:
+        return None, None, None, None
+    logits, tokens, stats, entropy, top_tokens = ctx.saved_tensors
+    dx = token_logprobs_bwd(logits, tokens, ctx.top, ctx.ignore_index, stats, entropy, top_tokens, dlogprob, dentropy,
+                            dtop)
+    return dx, None, None, None
+
+
+torch.library.register_autograd("ulm::token_logprobs", _token_logprobs_backward, setup_context=_token_logprobs_setup)
+
+
+def _check_tokens(tokens):
+    if not isinstance(tokens, torch.Tensor):
+        raise TypeError("tokens must be a tensor")
+    if tokens.is_floating_point() or tokens.is_complex() or tokens.dtype == torch.bool:
+        raise TypeError(f"tokens must be an integer tensor, got {tokens.dtype}")
+
+
+def token_logprobs(logits, tokens, top=0, ignore_index=-1):
+    """Log probabilities of `tokens` (...) under `logits` (..., V), as TokenLogprobs:
+
+      logprob      (...)      x_t - ln sum_i exp(x_i), t the token; 0, without a gradient, where t is
+                              ignore_index (F.cross_entropy's, -1 as in UnifiedLM.forward); NaN for any
+                              other token outside [0, V)
+      entropy      (...)      -sum_i p_i ln p_i
+      top_logprobs (..., top) the `top` most likely tokens' log probabilities (at most 64),
+      top_tokens   (..., top) and those tokens, the lower first on ties
+
+    fp32 from fp32, bf16 or fp16 logits, differentiable in them through the first three (dlogits in the
+    logits' dtype). Masked logits (-inf) have probability 0; a row of nothing else has logprob and
+    top_logprobs -inf, entropy 0 and no gradient. Any view whose last dimension is dense is read in
+    place (logits[:, :-1], say). The loss of a training step is -logprob summed over the tokens
+    that count."""
+    if not isinstance(logits, torch.Tensor):
+        raise TypeError("logits must be a tensor")
+    _check_float("logits", logits)
+    _check_tokens(tokens)
+    if logits.dim() < 1 or logits.shape[-1] == 0:
+        raise ValueError(f"logits must be (..., V), got {tuple(logits.shape)}")
+    if tokens.shape != logits.shape[:-1]:
+        raise ValueError(f"tokens {tuple(tokens.shape)} must have the logits' leading shape, {tuple(logits.shape)}")
+    most = min(logits.shape[-1], nat.lib().ulm_token_logprobs_max_top())
+    if not 0 <= top <= most:
+        raise ValueError(f"top must be between 0 and {most}, got {top}")
+    nat.dtype_code(logits.dtype)
+    nat.require_device(logits, tokens)
+    return TokenLogprobs(*token_logprobs_fwd(logits, tokens, top, ignore_index)[:4])
+
+
+# ---------------------------------------------------------------------------
+# embedding lookup with scaling (nn.Embedding, model.py:117, 150)
+
+@torch.library.custom_op("ulm::embed_fwd", mutates_args=())
+def embed_fwd(weight: Tensor, tokens: Tensor, scale: float) -> Tensor:
+    """scale W[tokens] (..., D) in the weight's dtype: ulm_embed_fwd."""
+    V, D = weight.shape
+    out = torch.empty(*tokens.shape, D, device=weight.device, dtype=weight.dtype)
+    if tokens.numel():
+        with torch.cuda.device(weight.device):
+            w, tok = weight.contiguous(), _int_tokens(tokens)
+            call("ulm_embed_fwd", ptr(w), nat.dtype_code(weight.dtype), ptr(tok), tok.numel(), V, D, scale, ptr(out),
+                 nat.stream_of(weight))
+    return out
+
+
+@embed_fwd.register_fake
+def _embed_fwd_fake(weight, tokens, scale):
+    return weight.new_empty(*tokens.shape, weight.shape[1])
+
+
+@torch.library.custom_op("ulm::embed_bwd", mutates_args=())
+def embed_bwd(dout: Tensor, tokens: Tensor, V: int, scale: float) -> Tensor:
+    """The weight's gradient (V, D) in dout's dtype: ulm_embed_bwd."""
+    D = dout.shape[-1]
+    dw = torch.empty(V, D, device=dout.device, dtype=dout.dtype)
+    if not tokens.numel():
+        return dw.zero_()
+    with torch.cuda.device(dout.device):
+        d, tok = dout.contiguous(), _int_tokens(tokens)
+        ws_bytes = nat.lib().ulm_embed_bwd_workspace_bytes(tok.numel(), V, D)
+        ws = torch.empty(max(ws_bytes, 1), device=dout.device, dtype=torch.uint8)
+        call("ulm_embed_bwd", ptr(d), nat.dtype_code(dout.dtype), ptr(tok), tok.numel(), V, D, scale, ptr(dw), ptr(ws),
+             ws_bytes, nat.stream_of(dout))
+    return dw
+
+
+@embed_bwd.register_fake
+def _embed_bwd_fake(dout, tokens, V, scale):
+    return dout.new_empty(V, dout.shape[-1])
+
+
+def _embed_setup(ctx, inputs, output):
+    weight, tokens, ctx.scale = inputs
+    ctx.V, ctx.dtype = weight.shape[0], weight.dtype
+    ctx.save_for_backward(tokens)
+    ctx.set_materialize_grads(False)
+
+
+def _embed_backward(ctx, dout):
+    if dout is None:
+        return None, None, None
+    tokens, = ctx.saved_tensors
+    return embed_bwd(dout.to(ctx.dtype), tokens, ctx.V, ctx.scale), None, None
+
+
+torch.library.register_autograd("ulm::embed_fwd", _embed_backward, setup_context=_embed_setup)
+
+
+def embedding(weight, tokens, scale=1.0):
+    """scale * weight[tokens]: weight (V, D) fp32, bf16 or fp16, tokens (...) integer, the result
+    (..., D) in the weight's dtype, rounded once. A token outside [0, V) gives a row of NaN.
+    The weight's gradient is dense, in its dtype: each row the fp32 sum of its tokens' gradients in
+    their order, so that equal inputs give equal bits; tokens outside [0, V) add nothing."""
+    if not isinstance(weight, torch.Tensor):
+        raise TypeError("weight must be a tensor")
+    if isinstance(scale, torch.Tensor):
+        raise TypeError("scale must be a number")
+    _check_float("weight", weight)
+    _check_tokens(tokens)
+    if weight.dim() != 2 or weight.numel() == 0:
+        raise ValueError(f"weight must be a non-empty (V, D), got {tuple(weight.shape)}")
+    if weight.shape[0] > 1 << 30 or tokens.numel() > 1 << 30:
+        raise ValueError(f"at most 2^30 tokens: weight {tuple(weight.shape)}, {tokens.numel()} tokens")
+    nat.dtype_code(weight.dtype)
+    nat.require_device(weight, tokens)
+    return embed_fwd(weight, tokens, float(scale))
+
+
+# ---------------------------------------------------------------------------
+# the gradients' global norm and clipping (train.py, before the optimizer's step)
+
+def _norm_type(norm_type):
+    code = nat.NORM_TYPES.get(float(norm_type))
+    if code is None:
+        raise ValueError(f"norm_type must be 2 or inf, got {norm_type}")
+    return code
+
+
+def _check_grads(grads, what="gradient"):
+    """The tensors of a norm: a tensor or an iterable of them, on one device, of the three types."""
+    grads = [grads] if isinstance(grads, torch.Tensor) else list(grads)
+    for t in grads:
+        if not isinstance(t, torch.Tensor):
+            raise TypeError(f"every {what} must be a tensor, got {type(t).__name__}")
+        if t.layout != torch.strided:
+            raise TypeError(f"every {what} must be strided, got {t.layout}")
+        nat.dtype_code(t.dtype)
+    nat.require_device(*grads)
+    return grads
+
+
+def _dense(t):
+    """Whether t's elements fill one region of memory, each once."""
+    if t.is_contiguous():
+        return True
+    want = 1
+    for st, n in sorted((st, n) for n, st in zip(t.shape, t.stride()) if n != 1):
+        if st != want:
+            return False
+        want *= n
+    return True
+
+
+def _table(pairs):
+    table = (nat.Grad * max(1, len(pairs)))()
+    for g, (src, dst) in zip(table, pairs):
+        g.src, g.numel, g.src_dtype = src.data_ptr(), src.numel(), nat.dtype_code(src.dtype)
+        if dst is not None:
+            g.dst, g.dst_dtype = dst.data_ptr(), nat.dtype_code(dst.dtype)
+    return table
+
+
+def _run_norm(entry, pairs, device, code, *bound):
+    norm = torch.empty((), device=device, dtype=torch.float32)
+    table = _table(pairs)
+    ws_bytes = nat.lib().ulm_grad_norm_workspace_bytes(table, len(pairs))
+    ws = torch.empty(ws_bytes, device=device, dtype=torch.uint8)
+    call(entry, table, len(pairs), code, *bound, ptr(norm), ptr(ws), ws_bytes, nat.stream_of(norm))
+    return norm
+
+
+@torch.no_grad()
+def grad_norm(grads, norm_type=2.0):
+    """The norm of all elements of `grads` (a tensor or an iterable of them) taken together, a 0-d fp32
+    tensor: the root of the sum of squares, summed in double, or with norm_type inf the largest |g|."""
+    code = _norm_type(norm_type)
+    grads = _check_grads(grads)
+    if not grads:
+        return torch.zeros(())
+    with torch.cuda.device(grads[0].device):
+        return _run_norm("ulm_grad_norm", [(t if _dense(t) else t.contiguous(), None) for t in grads],
+                         grads[0].device, code)
+
+
+def _check_regions(grads, out):
+    """Refuses results whose memory, from the first element to the last, overlaps
+    another result's or another gradient's."""
+    spans = []
+    for g, o in zip(grads, out):
+        if o.numel() == 0:
+            continue
+        if any(st == 0 and n > 1 for n, st in zip(o.shape, o.stride())):
+            raise ValueError("a result's elements share memory")
+        span = lambda t: (t.data_ptr(), t.data_ptr() + t.element_size() * (  # noqa: E731
+            1 + sum((n - 1) * st for n, st in zip(t.shape, t.stride()))))
+        spans.append((*span(o), True))
+        if g is not o and (g.data_ptr() != o.data_ptr() or g.dtype != o.dtype or g.stride() != o.stride()):
+            spans.append((*span(g), False))
+    written = read = 0
+    for start, end, is_out in sorted(spans):
+        if start < written or (is_out and start < read):
+            raise ValueError("results must not share memory with each other or with other gradients")
+        written = max(written, end) if is_out else written
+        read = max(read, end)
+
+
+@torch.no_grad()
+def clip_grads(grads, max_norm, out=None, norm_type=2.0):
+    """(norm, clipped): the norm of all `grads` (grad_norm) and every gradient times
+    min(1, max_norm / (norm + 1e-6)), in fp32 and rounded once to the result's dtype. `out` is a list of
+    tensors of the gradients' shapes to write, each of the three types (gradients in bf16 clipped into
+    the optimizer's fp32 buffers, say); out = grads clips in place, leaving the gradients as they
+    are where the norm is within the bound; None makes new tensors of the gradients' dtypes.
+    Nothing waits for the GPU. A NaN among the gradients makes the norm and all of them NaN."""
+    code = _norm_type(norm_type)
+    max_norm = float(max_norm)
+    if not max_norm >= 0.0:
+        raise ValueError(f"max_norm must not be negative, got {max_norm}")
+    in_place = out is grads
+    grads = _check_grads(grads)
+    if out is None:
+        out = [torch.empty_like(t) for t in grads]
+    else:
+        out = grads if in_place else _check_grads(out, "result")
+    if len(out) != len(grads) or any(o.shape != g.shape for o, g in zip(out, grads)):
+        raise ValueError("out must hold a tensor of each gradient's shape")
+    if not grads:
+        return torch.zeros(()), out
+    nat.require_device(*grads, *out)
+    _check_regions(grads, out)
+    with torch.cuda.device(grads[0].device):
+        pairs, late = [], []
+        for g, o in zip(grads, out):
+            if _dense(o) and g.stride() == o.stride():
+                pairs.append((g, o))
+                continue
+            src = g.contiguous()
+            dst = o if o.is_contiguous() else torch.empty_like(o, memory_format=torch.contiguous_format)
+            if dst is not o:
+                late.append((o, dst))
+            pairs.append((src, dst))
+        norm = _run_norm("ulm_clip_grads", pairs, grads[0].device, code, max_norm)
+        for o, dst in late:
+            o.copy_(dst)
+    return norm, out
+
+
+@torch.no_grad()
+def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=False):
+    """The gradients of `parameters` (a tensor or an iterable; those without one are passed over) clipped
+    in place to a joint norm of max_norm (clip_grads); returns the norm they had. With
+    error_if_nonfinite, a norm that is not finite raises before anything is changed (this waits for the GPU)."""
+    parameters = [parameters] if isinstance(parameters, torch.Tensor) else parameters
+    grads = [p.grad for p in parameters if p.grad is not None]
+    if error_if_nonfinite:
+        norm = grad_norm(grads, norm_type)
+        if not math.isfinite(norm.item()):
+            raise RuntimeError(f"the gradients' norm is {norm.item()}; nothing was clipped")
+    return clip_grads(grads, max_norm, out=grads, norm_type=norm_type)[0]

@@ -16,7 +16,16 @@ ULM_OK, ULM_ERR_INVALID, ULM_ERR_UNSUPPORTED, ULM_ERR_LAUNCH = 0, 1, 2, 3
 ULM_F32, ULM_BF16, ULM_F16 = 0, 1, 2
 DTYPE_CODE = {torch.float32: ULM_F32, torch.bfloat16: ULM_BF16, torch.float16: ULM_F16}
 
-P, I, SZ, F = ctypes.c_void_p, ctypes.c_int, ctypes.c_size_t, ctypes.c_float
+P, I, SZ, F, L = ctypes.c_void_p, ctypes.c_int, ctypes.c_size_t, ctypes.c_float, ctypes.c_longlong
+
+
+class Grad(ctypes.Structure):
+    """ulm_grad: one tensor of ulm_grad_norm / ulm_clip_grads."""
+    _fields_ = [("src", P), ("dst", P), ("numel", L), ("src_dtype", I), ("dst_dtype", I)]
+
+
+NORM_TYPES = {2.0: 2, float("inf"): 0}   # ULM_NORM_*
+
 
 # name -> (restype, argtypes); must match include/ulm_fm.h
 SIGNATURES = {
@@ -61,6 +70,16 @@ SIGNATURES = {
     "ulm_decode_flush": (I, [P, P, P, I, P, P, P, P, P, I, I, I, P]),
     "ulm_decode_step_workspace_bytes": (SZ, [I, I, I, I]),
     "ulm_decode_step": (I, [P, I, P, P, P, SZ, I, I, I, I, P]),
+    "ulm_token_logprobs_max_top": (I, []),
+    "ulm_token_logprobs_workspace_bytes": (SZ, [L, I, I]),
+    "ulm_token_logprobs": (I, [P, I, P, L, L, L, L, I, I, L, P, P, P, P, P, P, SZ, P]),
+    "ulm_token_logprobs_bwd": (I, [P, I, P, L, L, L, L, I, I, L, P, P, P, P, P, P, P, P]),
+    "ulm_embed_fwd": (I, [P, I, P, L, I, I, F, P, P]),
+    "ulm_embed_bwd_workspace_bytes": (SZ, [L, I, I]),
+    "ulm_embed_bwd": (I, [P, I, P, L, I, I, F, P, P, SZ, P]),
+    "ulm_grad_norm_workspace_bytes": (SZ, [P, I]),
+    "ulm_grad_norm": (I, [P, I, I, P, P, SZ, P]),
+    "ulm_clip_grads": (I, [P, I, I, F, P, P, SZ, P]),
     "ulm_la_timer_start": (I, [I]),
     "ulm_la_timer_stop": (I, [ctypes.POINTER(ctypes.c_double), ctypes.POINTER(ctypes.c_int)]),
     "ulm_la_timer_product": (I, [I, ctypes.POINTER(ctypes.c_double), ctypes.POINTER(ctypes.c_int)]),
