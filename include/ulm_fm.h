@@ -397,7 +397,8 @@ int ulm_decode_step(const ulm_decode_layer *layers, int n_layers, const float *x
  *   top_logprobs (rows, top) out: the `top` largest entries' log probabilities,
  *   top_tokens   (rows, top) out: and their indices; the lower index first on ties, a NaN
  *                            above all numbers. top at most ulm_token_logprobs_max_top() and V
- *   stats        (rows, 2)   out: the row's maximum and ln sum_i e^(x_i - max), for the backward
+ *   stats        (rows, 2)   out: the row's maximum and ln sum_i e^(x_i - max), for the backward;
+ *                            NULL: not wanted
  * A row of -inf only has logprob and top_logprobs -inf (0 if ignored), entropy 0, top_tokens
  * 0, 1, .. and gradient 0. A row with a NaN or +inf has NaN throughout (but for top_tokens and
  * an ignored token's 0). Workspace of ulm_token_logprobs_workspace_bytes() bytes (may be 0: few

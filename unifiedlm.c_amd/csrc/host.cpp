@@ -14,13 +14,17 @@
 // subclasses, disagreeing shapes, other dtypes and devices.
 #include <ATen/ATen.h>
 #include <ATen/core/dispatch/Dispatcher.h>
+#include <c10/core/DeviceGuard.h>
 #include <c10/core/impl/LocalDispatchKeySet.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/python_variable.h>
+#include <torch/csrc/autograd/variable.h>
 #include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/csrc/utils/pybind.h>
 
+#include <algorithm>
+#include <limits>
 #include <optional>
 #include <string>
 #include <vector>
@@ -522,6 +526,358 @@ py::object decode_step(const py::handle &x_, const py::list &states, const py::l
     return py::cast(out);
 }
 
+// ---- the ends of a step: token log probabilities, embedding, gradient clipping
+
+// a Tensor or Parameter proper, strided, on a GPU, of an integer type; undefined otherwise
+Tensor plain_ids(const py::handle &h) {
+    if (!THPVariable_CheckExact(h.ptr())) return {};
+    const Tensor &t = THPVariable_Unpack(h.ptr());
+    if (!t.defined() || !t.is_cuda() || t.layout() != at::kStrided || !at::isIntegralType(t.scalar_type(), false) ||
+        t.key_set().has_any(kNotPlain))
+        return {};
+    return t;
+}
+Tensor ids64(const Tensor &t) { return (t.scalar_type() == at::kLong ? t : t.to(at::kLong)).contiguous(); }
+const long long *ip(const Tensor &t) { return static_cast<const long long *>(t.data_ptr()); }
+
+// kernel._rows: the rows of (..., V) logits as the kernels address them, copied where they cannot
+struct LogitRows {
+    Tensor x;
+    int64_t rows, inner = 1, outer_stride = 0, row_stride;
+    int V;
+    explicit LogitRows(const Tensor &t) : x(t), V(static_cast<int>(t.size(-1))) {
+        rows = t.numel() / V;
+        row_stride = V;
+        int groups = 0;
+        int64_t n[2] = {1, 1}, st[2] = {0, V};
+        bool ok = V == 1 || t.stride(-1) == 1;
+        for (int64_t d = 0; ok && d + 1 < t.dim(); ++d) {
+            if (t.size(d) == 1) continue;
+            if (groups && st[groups - 1] == t.size(d) * t.stride(d)) {
+                n[groups - 1] *= t.size(d);
+                st[groups - 1] = t.stride(d);
+            } else if (groups == 2) {
+                ok = false;
+            } else {
+                n[groups] = t.size(d);
+                st[groups++] = t.stride(d);
+            }
+        }
+        if (!ok) {
+            x = t.contiguous();
+            inner = std::max<int64_t>(rows, 1);
+        } else if (groups) {
+            inner = n[groups - 1];
+            row_stride = st[groups - 1];
+            if (groups == 2) outer_stride = st[0];
+        }
+    }
+};
+
+// A leaf that an eager graph still holds has its gradient's accumulation tied to that graph's stream; a capture on
+// another one that goes through it ends the process inside the runtime. Refused where it can be seen.
+void check_capture(const Tensor &leaf) {
+    if (!leaf.requires_grad() || !leaf.is_leaf() || !at::GradMode::is_enabled()) return;
+    hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+    const auto now = c10::hip::getCurrentHIPStream(leaf.get_device());
+    if (hipStreamIsCapturing(now.stream(), &status) != hipSuccess || status == hipStreamCaptureStatusNone) return;
+    const auto node = torch::autograd::impl::try_get_grad_accumulator(leaf);
+    TORCH_CHECK(!node || !node->stream() || node->stream()->id() == now.id(),
+                "captured while an eager graph of the same leaf is alive on another stream: let go of that graph's outputs first");
+}
+
+struct TokenLogprobs : torch::autograd::Function<TokenLogprobs> {
+    // (logprob, entropy, top_logprobs, top_tokens); the statistics too where `stats` is given
+    static variable_list compute(const Tensor &logits, const Tensor &tok, int64_t top, int64_t ignore, Tensor *stats) {
+        const c10::DeviceGuard device(logits.device());
+        const Maker make(logits);
+        const auto lead = logits.sizes().slice(0, logits.dim() - 1);
+        std::vector<int64_t> with(lead.begin(), lead.end());
+        with.push_back(top);
+        const Tensor logprob = make(lead), entropy = make(lead), top_lp = make(with), top_tok = make(with, at::kLong);
+        const LogitRows r(logits);
+        if (stats) {
+            with.back() = 2;
+            *stats = make(with);
+        }
+        if (r.rows) {
+            const size_t wb = ulm_token_logprobs_workspace_bytes(r.rows, r.V, top);
+            const Tensor ws = wb ? make.bytes(wb) : Tensor();
+            check("ulm_token_logprobs",
+                  ulm_token_logprobs(r.x.data_ptr(), code(logits.scalar_type()), ip(tok), r.rows, r.inner, r.outer_stride,
+                                     r.row_stride, r.V, top, ignore, fpm(logprob), fpm(entropy), fpm(top_lp),
+                                     static_cast<long long *>(top_tok.data_ptr()), stats ? fpm(*stats) : nullptr,
+                                     wb ? ws.data_ptr() : nullptr, wb, stream_of(logits)));
+        }
+        return {logprob, entropy, top_lp, top_tok};
+    }
+    static variable_list forward(AutogradContext *ctx, const Tensor &logits, const Tensor &tokens, int64_t top, int64_t ignore) {
+        at::AutoDispatchBelowAutograd guard;
+        Tensor stats;
+        variable_list out = compute(logits, ids64(tokens), top, ignore, &stats);
+        ctx->save_for_backward({logits, tokens, stats, out[1], out[3]});
+        ctx->saved_data["top"] = top;
+        ctx->saved_data["ignore"] = ignore;
+        ctx->mark_non_differentiable({out[3]});
+        ctx->set_materialize_grads(false);
+        return out;
+    }
+    static variable_list backward(AutogradContext *ctx, variable_list grads) {
+        variable_list out(4);
+        if (!grads[0].defined() && !grads[1].defined() && !grads[2].defined()) return out;
+        const auto sv = ctx->get_saved_variables();
+        const Tensor &logits = sv[0], &tokens = sv[1], &stats = sv[2], &entropy = sv[3], &top_tok = sv[4];
+        const int64_t top = ctx->saved_data["top"].toInt(), ignore = ctx->saved_data["ignore"].toInt();
+        grads.resize(3);
+        if (!launches(grads, sv)) {
+            using O = const std::optional<Tensor> &;
+            using F = Tensor(const Tensor &, const Tensor &, c10::SymInt, c10::SymInt, const Tensor &, const Tensor &,
+                             const Tensor &, O, O, O);
+            auto opt = [](const Tensor &t) { return t.defined() ? std::optional<Tensor>(t) : std::nullopt; };
+            out[0] = registered<F>("ulm::token_logprobs_bwd").call(logits, tokens, top, ignore, stats, entropy, top_tok, opt(grads[0]),
+                                                                   opt(grads[1]), opt(grads[2]));
+            return out;
+        }
+        at::AutoDispatchBelowAutograd guard;
+        const c10::DeviceGuard device(logits.device());
+        const Maker make(logits);
+        out[0] = make(logits.sizes(), logits.scalar_type());
+        const LogitRows r(logits);
+        if (r.rows == 0) return out;
+        const Tensor tok = ids64(tokens), st = stats.contiguous(), H = entropy.contiguous(), tt = top_tok.contiguous();
+        Tensor up[3];
+        for (int i = 0; i < 3; ++i)
+            if (grads[i].defined() && grads[i].numel()) up[i] = f32c(grads[i]);
+        check("ulm_token_logprobs_bwd",
+              ulm_token_logprobs_bwd(r.x.data_ptr(), code(logits.scalar_type()), ip(tok), r.rows, r.inner, r.outer_stride, r.row_stride,
+                                     r.V, top, ignore, fp(st), fp(H), ip(tt), fp(up[0]), fp(up[1]), fp(up[2]), out[0].data_ptr(),
+                                     stream_of(logits)));
+        return out;
+    }
+};
+
+bool wants_grad(const Tensor &t) { return t.requires_grad() && at::GradMode::is_enabled(); }
+
+py::object token_logprobs(const py::handle &logits_, const py::handle &tokens_, const py::handle &top_, const py::handle &ignore_) {
+    if (!plain_thread() || !PyLong_CheckExact(top_.ptr()) || !PyLong_CheckExact(ignore_.ptr())) return py::none();
+    const Tensor logits = plain(logits_), tokens = plain_ids(tokens_);
+    if (!logits.defined() || !tokens.defined() || !has_code(logits) || logits.device() != tokens.device() || logits.dim() < 1 ||
+        logits.size(-1) == 0 || logits.size(-1) > INT32_MAX || tokens.sizes() != logits.sizes().slice(0, logits.dim() - 1))
+        return py::none();
+    const int64_t top = top_.cast<int64_t>(), ignore = ignore_.cast<int64_t>();
+    if (top < 0 || top > std::min<int64_t>(logits.size(-1), ulm_token_logprobs_max_top())) return py::none();
+    const variable_list out = unlocked([&] {
+        if (wants_grad(logits)) {
+            check_capture(logits);
+            return TokenLogprobs::apply(logits, tokens, top, ignore);
+        }
+        at::AutoDispatchBelowAutograd guard;
+        return TokenLogprobs::compute(logits, ids64(tokens), top, ignore, nullptr);
+    });
+    return py::make_tuple(py::cast(out[0]), py::cast(out[1]), py::cast(out[2]), py::cast(out[3]));
+}
+
+struct Embedding : torch::autograd::Function<Embedding> {
+    static Tensor compute(const Tensor &weight, const Tensor &tokens, double scale) {
+        const c10::DeviceGuard device(weight.device());
+        std::vector<int64_t> shape(tokens.sizes().begin(), tokens.sizes().end());
+        shape.push_back(weight.size(1));
+        const Tensor out = Maker(weight)(shape, weight.scalar_type());
+        if (tokens.numel()) {
+            const Tensor w = weight.contiguous(), tok = ids64(tokens);
+            check("ulm_embed_fwd", ulm_embed_fwd(w.data_ptr(), code(w.scalar_type()), ip(tok), tok.numel(), w.size(0), w.size(1),
+                                                 static_cast<float>(scale), out.data_ptr(), stream_of(w)));
+        }
+        return out;
+    }
+    static Tensor forward(AutogradContext *ctx, const Tensor &weight, const Tensor &tokens, double scale) {
+        at::AutoDispatchBelowAutograd guard;
+        ctx->save_for_backward({tokens});
+        ctx->saved_data["scale"] = scale;
+        ctx->saved_data["V"] = weight.size(0);
+        ctx->saved_data["dtype"] = static_cast<int64_t>(weight.scalar_type());
+        ctx->set_materialize_grads(false);
+        return compute(weight, tokens, scale);
+    }
+    static variable_list backward(AutogradContext *ctx, variable_list grads) {
+        if (!grads[0].defined()) return variable_list(3);
+        const auto sv = ctx->get_saved_variables();
+        const double scale = ctx->saved_data["scale"].toDouble();
+        const int64_t V = ctx->saved_data["V"].toInt();
+        const auto dt = static_cast<at::ScalarType>(ctx->saved_data["dtype"].toInt());
+        if (!launches(grads, sv)) {
+            using F = Tensor(const Tensor &, const Tensor &, c10::SymInt, double);
+            return {registered<F>("ulm::embed_bwd").call(grads[0].to(dt), sv[0], V, scale), Tensor(), Tensor()};
+        }
+        at::AutoDispatchBelowAutograd guard;
+        const c10::DeviceGuard device(grads[0].device());
+        const Tensor dout = cast(grads[0], dt), tok = ids64(sv[0]);
+        const int64_t D = dout.size(-1), N = tok.numel();
+        const Maker make(dout);
+        if (N == 0) return {at::zeros({V, D}, make.opt.dtype(dt)), Tensor(), Tensor()};
+        const Tensor dw = make({V, D}, dt);
+        const size_t wb = ulm_embed_bwd_workspace_bytes(N, V, D);
+        const Tensor ws = make.bytes(wb);
+        check("ulm_embed_bwd", ulm_embed_bwd(dout.data_ptr(), code(dt), ip(tok), N, V, D, static_cast<float>(scale), dw.data_ptr(),
+                                             ws.data_ptr(), wb, stream_of(dout)));
+        return {dw, Tensor(), Tensor()};
+    }
+};
+
+py::object embedding(const py::handle &weight_, const py::handle &tokens_, const py::handle &scale_) {
+    if (!plain_thread() || !(PyFloat_CheckExact(scale_.ptr()) || PyLong_CheckExact(scale_.ptr()))) return py::none();
+    const Tensor weight = plain(weight_), tokens = plain_ids(tokens_);
+    if (!weight.defined() || !tokens.defined() || !has_code(weight) || weight.device() != tokens.device() || weight.dim() != 2 ||
+        weight.numel() == 0 || weight.size(0) > (1 << 30) || tokens.numel() > (1 << 30) || weight.size(1) > (1 << 24))
+        return py::none();
+    const double scale = scale_.cast<double>();
+    return py::cast(unlocked([&] {
+        if (wants_grad(weight)) {
+            check_capture(weight);
+            return Embedding::apply(weight, tokens, scale);
+        }
+        at::AutoDispatchBelowAutograd guard;
+        return Embedding::compute(weight, tokens, scale);
+    }));
+}
+
+// the plain tensors of a list or tuple, all of the three types and on one device; false otherwise
+bool plain_list(const py::handle &list, std::vector<Tensor> &out) {
+    if (!PyList_CheckExact(list.ptr()) && !PyTuple_CheckExact(list.ptr())) return false;
+    const Py_ssize_t n = PySequence_Fast_GET_SIZE(list.ptr());
+    out.reserve(n);
+    for (Py_ssize_t i = 0; i < n; ++i) {
+        out.push_back(plain(PySequence_Fast_GET_ITEM(list.ptr(), i)));
+        const Tensor &t = out.back();
+        if (!t.defined() || !has_code(t) || t.device() != out[0].device()) return false;
+    }
+    return n > 0;
+}
+
+// 0 for a maximum norm, 2 for the root of the squares, -1 for what the Python implementation refuses
+int norm_code(const py::handle &h) {
+    if (!PyFloat_CheckExact(h.ptr()) && !PyLong_CheckExact(h.ptr())) return -1;
+    const double v = h.cast<double>();
+    return v == 2.0 ? ULM_NORM_2 : v == std::numeric_limits<double>::infinity() ? ULM_NORM_INF : -1;
+}
+
+ulm_grad entry(const Tensor &src, const Tensor &dst) {
+    return {src.data_ptr(), dst.defined() ? dst.data_ptr() : nullptr, src.numel(), code(src.scalar_type()),
+            dst.defined() ? code(dst.scalar_type()) : ULM_F32};
+}
+
+Tensor run_norm(const std::vector<ulm_grad> &table, const Tensor &like, int norm, const float *bound) {
+    const Maker make(like);
+    const Tensor out = make({});
+    const size_t wb = ulm_grad_norm_workspace_bytes(table.data(), table.size());
+    const Tensor ws = make.bytes(wb);
+    if (bound)
+        check("ulm_clip_grads", ulm_clip_grads(table.data(), table.size(), norm, *bound, fpm(out), ws.data_ptr(), wb, stream_of(like)));
+    else
+        check("ulm_grad_norm", ulm_grad_norm(table.data(), table.size(), norm, fpm(out), ws.data_ptr(), wb, stream_of(like)));
+    return out;
+}
+
+py::object grad_norm(const py::handle &grads_, const py::handle &norm_type) {
+    std::vector<Tensor> grads;
+    const int norm = norm_code(norm_type);
+    if (!plain_thread() || norm < 0 || !plain_list(grads_, grads)) return py::none();
+    return py::cast(unlocked([&] {
+        at::AutoDispatchBelowAutograd guard;
+        const c10::DeviceGuard device(grads[0].device());
+        std::vector<ulm_grad> table;
+        for (Tensor &t : grads) {
+            if (!t.is_non_overlapping_and_dense()) t = t.contiguous();
+            table.push_back(entry(t, Tensor()));
+        }
+        return run_norm(table, grads[0], norm, nullptr);
+    }));
+}
+
+// The norm of `grads`, clipped into `out`; undefined where the Python implementation decides: results that are not one
+// region each in their gradients' order, or that overlap another one's or another gradient's (kernel._check_regions).
+Tensor clip(const std::vector<Tensor> &grads, const std::vector<Tensor> &out, double bound, int norm) {
+    struct Span {
+        uintptr_t from, to;
+        bool written;
+    };
+    std::vector<Span> spans;
+    std::vector<ulm_grad> table;
+    for (size_t i = 0; i < grads.size(); ++i) {
+        const Tensor &g = grads[i], &o = out[i];
+        if (!g.is_non_overlapping_and_dense() || g.sizes() != o.sizes() || g.strides() != o.strides()) return {};
+        table.push_back(entry(g, o));
+        if (g.numel() == 0) continue;
+        const auto from = reinterpret_cast<uintptr_t>(o.data_ptr()), src = reinterpret_cast<uintptr_t>(g.data_ptr());
+        spans.push_back({from, from + o.nbytes(), true});
+        if (src != from || g.scalar_type() != o.scalar_type()) spans.push_back({src, src + g.nbytes(), false});
+    }
+    std::sort(spans.begin(), spans.end(), [](const Span &a, const Span &b) { return a.from < b.from; });
+    uintptr_t written = 0, read = 0;
+    for (const Span &s : spans) {
+        if (s.from < written || (s.written && s.from < read)) return {};
+        if (s.written) written = std::max(written, s.to);
+        read = std::max(read, s.to);
+    }
+    at::AutoDispatchBelowAutograd guard;
+    const c10::DeviceGuard device(grads[0].device());
+    const float b = static_cast<float>(bound);
+    const Tensor n = run_norm(table, grads[0], norm, &b);
+    for (const Tensor &o : out)
+        if (!o.is_inference()) o.unsafeGetTensorImpl()->bump_version();   // written behind autograd's back
+    return n;
+}
+
+py::object clip_grads(const py::handle &grads_, const py::handle &max_norm, const py::handle &out_, const py::handle &norm_type) {
+    std::vector<Tensor> grads, out;
+    const int norm = norm_code(norm_type);
+    if (!plain_thread() || norm < 0 || !(PyFloat_CheckExact(max_norm.ptr()) || PyLong_CheckExact(max_norm.ptr()))) return py::none();
+    const double bound = max_norm.cast<double>();
+    if (!(bound >= 0) || !plain_list(grads_, grads)) return py::none();
+    const bool fresh = out_.is_none();
+    if (out_.ptr() == grads_.ptr()) out = grads;
+    else if (!fresh && (!plain_list(out_, out) || out.size() != grads.size() || out[0].device() != grads[0].device())) return py::none();
+    const Tensor n = unlocked([&] {
+        if (fresh)
+            for (const Tensor &g : grads) {
+                at::NoGradGuard no_grad;
+                out.push_back(at::empty_like(g));
+            }
+        return clip(grads, out, bound, norm);
+    });
+    if (!n.defined()) return py::none();
+    py::list res;
+    for (size_t i = 0; i < out.size(); ++i)
+        res.append(fresh ? py::cast(out[i]) : py::reinterpret_borrow<py::object>(PySequence_Fast_GET_ITEM(out_.ptr(), i)));
+    return py::make_tuple(py::cast(n), res);
+}
+
+// clip_grad_norm_ over a list or tuple of parameters, in place
+py::object clip_parameters(const py::handle &params, const py::handle &max_norm, const py::handle &norm_type) {
+    const int norm = norm_code(norm_type);
+    if (!plain_thread() || norm < 0 || !(PyFloat_CheckExact(max_norm.ptr()) || PyLong_CheckExact(max_norm.ptr())) ||
+        !(PyList_CheckExact(params.ptr()) || PyTuple_CheckExact(params.ptr())))
+        return py::none();
+    const double bound = max_norm.cast<double>();
+    std::vector<Tensor> grads;
+    const Py_ssize_t n = PySequence_Fast_GET_SIZE(params.ptr());
+    for (Py_ssize_t i = 0; i < n; ++i) {
+        PyObject *p = PySequence_Fast_GET_ITEM(params.ptr(), i);
+        if (!THPVariable_CheckExact(p)) return py::none();
+        const Tensor &t = THPVariable_Unpack(p);
+        if (!t.defined() || !t.is_leaf()) return py::none();
+        const Tensor &g = t.grad();
+        if (!g.defined()) continue;
+        if (!g.is_cuda() || g.layout() != at::kStrided || !has_code(g) || g.key_set().has_any(kNotPlain) ||
+            (!grads.empty() && g.device() != grads[0].device()))
+            return py::none();
+        grads.push_back(g);
+    }
+    if (!(bound >= 0) || grads.empty()) return py::none();
+    const Tensor out = unlocked([&] { return clip(grads, grads, bound, norm); });
+    return out.defined() ? py::cast(out) : py::none();
+}
+
 }  // namespace
 
 PYBIND11_MODULE(ulm_host, m) {
@@ -530,4 +886,9 @@ PYBIND11_MODULE(ulm_host, m) {
     m.def("prefill", &prefill);
     m.def("copies", &copies);
     m.def("decode_step", &decode_step);
+    m.def("token_logprobs", &token_logprobs);
+    m.def("embedding", &embedding);
+    m.def("grad_norm", &grad_norm);
+    m.def("clip_grads", &clip_grads);
+    m.def("clip_parameters", &clip_parameters);
 }

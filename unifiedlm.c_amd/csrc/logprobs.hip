@@ -153,8 +153,10 @@ __device__ __forceinline__ void finish_row(const Rows &a, const Outs &o, long lo
     }
     o.logprob[r] = lp;
     o.entropy[r] = v.s == 0.f ? 0.f : logs - v.u / v.s;
-    o.stats[2 * r] = m;
-    o.stats[2 * r + 1] = logs;
+    if (o.stats) {
+        o.stats[2 * r] = m;
+        o.stats[2 * r + 1] = logs;
+    }
 }
 
 __device__ __forceinline__ void put_top(const Rows &a, const Outs &o, long long r, int rank, uint64_t key, float m, float logs) {
@@ -461,7 +463,7 @@ extern "C" int ulm_token_logprobs(const void *logits, int dtype, const long long
                                   float *logprob, float *entropy, float *top_logprobs, long long *top_tokens, float *stats,
                                   void *workspace, size_t workspace_bytes, void *stream) {
     ULM_TRY(check_rows("ulm_token_logprobs", rows, inner, V, top, dtype));
-    ULM_REQUIRE(logits && tokens && logprob && entropy && stats && (top == 0 || (top_logprobs && top_tokens)),
+    ULM_REQUIRE(logits && tokens && logprob && entropy && (top == 0 || (top_logprobs && top_tokens)),
                 "ulm_token_logprobs: null pointer");
     const int parts = lp::parts_of(rows, V);
     const size_t need = ulm_token_logprobs_workspace_bytes(rows, V, top);

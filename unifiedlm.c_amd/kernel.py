@@ -922,6 +922,10 @@ def token_logprobs(logits, tokens, top=0, ignore_index=-1):
     top_logprobs -inf, entropy 0 and no gradient. Any view whose last dimension is dense is read in
     place (logits[:, :-1], say). The loss of a training step is -logprob summed over the tokens
     that count."""
+    if _plain_eager():
+        out = nat.host().token_logprobs(logits, tokens, top, ignore_index)
+        if out is not None:
+            return TokenLogprobs._make(out)
     if not isinstance(logits, torch.Tensor):
         raise TypeError("logits must be a tensor")
     _check_float("logits", logits)
@@ -1002,6 +1006,10 @@ def embedding(weight, tokens, scale=1.0):
     (..., D) in the weight's dtype, rounded once. A token outside [0, V) gives a row of NaN.
     The weight's gradient is dense, in its dtype: each row the fp32 sum of its tokens' gradients in
     their order, so that equal inputs give equal bits; tokens outside [0, V) add nothing."""
+    if _plain_eager():
+        out = nat.host().embedding(weight, tokens, scale)
+        if out is not None:
+            return out
     if not isinstance(weight, torch.Tensor):
         raise TypeError("weight must be a tensor")
     if isinstance(scale, torch.Tensor):
@@ -1061,26 +1069,26 @@ def _table(pairs):
     return table
 
 
-def _run_norm(entry, pairs, device, code, *bound):
+def _run_norm(entry, pairs, device, norm_type, *bound):
     norm = torch.empty((), device=device, dtype=torch.float32)
     table = _table(pairs)
     ws_bytes = nat.lib().ulm_grad_norm_workspace_bytes(table, len(pairs))
     ws = torch.empty(ws_bytes, device=device, dtype=torch.uint8)
-    call(entry, table, len(pairs), code, *bound, ptr(norm), ptr(ws), ws_bytes, nat.stream_of(norm))
+    call(entry, table, len(pairs), _norm_type(norm_type), *bound, ptr(norm), ptr(ws), ws_bytes, nat.stream_of(norm))
     return norm
 
 
-@torch.no_grad()
-def grad_norm(grads, norm_type=2.0):
-    """The norm of all elements of `grads` (a tensor or an iterable of them) taken together, a 0-d fp32
-    tensor: the root of the sum of squares, summed in double, or with norm_type inf the largest |g|."""
-    code = _norm_type(norm_type)
-    grads = _check_grads(grads)
-    if not grads:
-        return torch.zeros(())
+@torch.library.custom_op("ulm::grad_norm", mutates_args=())
+def _grad_norm_op(grads: list[Tensor], norm_type: float) -> Tensor:
+    """ulm_grad_norm over at least one tensor."""
     with torch.cuda.device(grads[0].device):
         return _run_norm("ulm_grad_norm", [(t if _dense(t) else t.contiguous(), None) for t in grads],
-                         grads[0].device, code)
+                         grads[0].device, norm_type)
+
+
+@_grad_norm_op.register_fake
+def _grad_norm_fake(grads, norm_type):
+    return grads[0].new_empty((), dtype=torch.float32)
 
 
 def _check_regions(grads, out):
@@ -1105,6 +1113,60 @@ def _check_regions(grads, out):
         read = max(read, end)
 
 
+def _clip_impl(grads, out, max_norm, norm_type):
+    _check_regions(grads, out)
+    with torch.cuda.device(grads[0].device):
+        pairs, late = [], []
+        for g, o in zip(grads, out):
+            if _dense(o) and g.stride() == o.stride():
+                pairs.append((g, o))
+                continue
+            src = g.contiguous()
+            dst = o if o.is_contiguous() else torch.empty_like(o, memory_format=torch.contiguous_format)
+            if dst is not o:
+                late.append((o, dst))
+            pairs.append((src, dst))
+        norm = _run_norm("ulm_clip_grads", pairs, grads[0].device, norm_type, max_norm)
+        for o, dst in late:
+            o.copy_(dst)
+    return norm
+
+
+@torch.library.custom_op("ulm::clip_grads", mutates_args={"out"})
+def _clip_op(grads: list[Tensor], out: list[Tensor], max_norm: float, norm_type: float) -> Tensor:
+    """ulm_clip_grads over at least one tensor, into `out`; returns the norm."""
+    return _clip_impl(grads, out, max_norm, norm_type)
+
+
+@torch.library.custom_op("ulm::clip_grads_", mutates_args={"grads"})
+def _clip_op_(grads: list[Tensor], max_norm: float, norm_type: float) -> Tensor:
+    """ulm_clip_grads over at least one tensor, in place; returns the norm."""
+    return _clip_impl(grads, grads, max_norm, norm_type)
+
+
+@_clip_op.register_fake
+def _clip_fake(grads, out, max_norm, norm_type):
+    return grads[0].new_empty((), dtype=torch.float32)
+
+
+@_clip_op_.register_fake
+def _clip_fake_(grads, max_norm, norm_type):
+    return grads[0].new_empty((), dtype=torch.float32)
+
+
+@torch.no_grad()
+def grad_norm(grads, norm_type=2.0):
+    """The norm of all elements of `grads` (a tensor or an iterable of them) taken together, a 0-d fp32
+    tensor: the root of the sum of squares, summed in double, or with norm_type inf the largest |g|."""
+    if _plain_eager():
+        out = nat.host().grad_norm(grads, norm_type)
+        if out is not None:
+            return out
+    _norm_type(norm_type)
+    grads = _check_grads(grads)
+    return _grad_norm_op(grads, float(norm_type)) if grads else torch.zeros(())
+
+
 @torch.no_grad()
 def clip_grads(grads, max_norm, out=None, norm_type=2.0):
     """(norm, clipped): the norm of all `grads` (grad_norm) and every gradient times
@@ -1112,8 +1174,14 @@ def clip_grads(grads, max_norm, out=None, norm_type=2.0):
     tensors of the gradients' shapes to write, each of the three types (gradients in bf16 clipped into
     the optimizer's fp32 buffers, say); out = grads clips in place, leaving the gradients as they
     are where the norm is within the bound; None makes new tensors of the gradients' dtypes.
-    Nothing waits for the GPU. A NaN among the gradients makes the norm and all of them NaN."""
-    code = _norm_type(norm_type)
+    Nothing waits for the GPU. A NaN among the gradients makes the norm and all of them NaN.
+    Results share no memory, from their first to their last elements, with each other or with
+    another gradient."""
+    if _plain_eager():
+        done = nat.host().clip_grads(grads, max_norm, out, norm_type)
+        if done is not None:
+            return done
+    _norm_type(norm_type)
     max_norm = float(max_norm)
     if not max_norm >= 0.0:
         raise ValueError(f"max_norm must not be negative, got {max_norm}")
@@ -1128,22 +1196,9 @@ def clip_grads(grads, max_norm, out=None, norm_type=2.0):
     if not grads:
         return torch.zeros(()), out
     nat.require_device(*grads, *out)
-    _check_regions(grads, out)
-    with torch.cuda.device(grads[0].device):
-        pairs, late = [], []
-        for g, o in zip(grads, out):
-            if _dense(o) and g.stride() == o.stride():
-                pairs.append((g, o))
-                continue
-            src = g.contiguous()
-            dst = o if o.is_contiguous() else torch.empty_like(o, memory_format=torch.contiguous_format)
-            if dst is not o:
-                late.append((o, dst))
-            pairs.append((src, dst))
-        norm = _run_norm("ulm_clip_grads", pairs, grads[0].device, code, max_norm)
-        for o, dst in late:
-            o.copy_(dst)
-    return norm, out
+    if in_place:
+        return _clip_op_(grads, max_norm, float(norm_type)), out
+    return _clip_op(grads, out, max_norm, float(norm_type)), out
 
 
 @torch.no_grad()
@@ -1151,10 +1206,14 @@ def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=Fals
     """The gradients of `parameters` (a tensor or an iterable; those without one are passed over) clipped
     in place to a joint norm of max_norm (clip_grads); returns the norm they had. With
     error_if_nonfinite, a norm that is not finite raises before anything is changed (this waits for the GPU)."""
-    parameters = [parameters] if isinstance(parameters, torch.Tensor) else parameters
-    grads = [p.grad for p in parameters if p.grad is not None]
+    parameters = [parameters] if isinstance(parameters, torch.Tensor) else list(parameters)
     if error_if_nonfinite:
-        norm = grad_norm(grads, norm_type)
+        norm = grad_norm([p.grad for p in parameters if p.grad is not None], norm_type)
         if not math.isfinite(norm.item()):
             raise RuntimeError(f"the gradients' norm is {norm.item()}; nothing was clipped")
+    if _plain_eager():
+        norm = nat.host().clip_parameters(parameters, max_norm, norm_type)
+        if norm is not None:
+            return norm
+    grads = [p.grad for p in parameters if p.grad is not None]
     return clip_grads(grads, max_norm, out=grads, norm_type=norm_type)[0]
