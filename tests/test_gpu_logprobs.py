@@ -205,16 +205,55 @@ def test_ties_go_to_the_lower_index(rows, dt):
 def test_largest_entries_all_in_a_few_threads(dt, V, vec, order):
     """More candidates than the list holds: the large entries lie where only a few threads read."""
     say(f"token_logprobs crowded candidates {dt} {order}")
-    rows = 513   # whole rows to a workgroup
+    rows = 513
     logits, tokens, _ = make(rows, V, dt, 19, std=0.5)
     where = torch.nonzero((torch.arange(V) // vec) % 64 < 8).flatten().cuda()
     n = where.numel()
     rise = torch.linspace(4, 30, n).cuda()
     logits[:, where] = {"rising": rise, "falling": rise.flip(0), "equal": torch.full_like(rise, 9.0)}[order].to(DT[dt])
     out = kernel.token_logprobs(logits, tokens, 64)
-    for r in (0, 512):
+    for r in (0, rows - 1):
         ids = torch.sort(logits[r].float(), descending=True, stable=True).indices[:64]
         assert torch.equal(out.top_tokens[r], ids)
+
+
+@pytest.mark.parametrize("dt", ["fp32", "bf16"])
+@pytest.mark.parametrize("rows", [1, 3, 2100])
+def test_many_ties_at_the_last_place(rows, dt):
+    """The top-th entry is one of thousands of equal ones, spread or at the row's end, with or without larger ones."""
+    say(f"token_logprobs thousands of ties rows={rows} {dt}")
+    V = 40000
+    logits, tokens, gen = make(rows, V, dt, 53, std=0.1)
+    logits.clamp_(max=0.0)          # half of them 0
+    logits[0, :V - 700] = -3.0      # equal ones at the end only
+    if rows > 1:
+        logits[1, torch.randperm(V, generator=gen)[:40].cuda()] = 2.5
+        logits[2] = -math.inf
+        logits[2, [5, 39999]] = 1.0
+        tokens[2] = 5
+    for top in (1, 17, 64):
+        out = kernel.token_logprobs(logits, tokens, top)
+        ids = torch.sort(logits[:3].float().cpu(), dim=-1, descending=True, stable=True).indices[:, :top]
+        assert torch.equal(out.top_tokens[:3].cpu(), ids)
+
+
+@pytest.mark.parametrize("rows", [1, 2100])
+def test_wide_rows_are_joined_from_parts(rows):
+    """More columns than one workgroup's table holds."""
+    say(f"token_logprobs wide rows={rows}")
+    gen = torch.Generator(device="cuda").manual_seed(59)
+    V = 200001 if rows == 1 else 70001
+    logits = torch.randn(rows, V, device="cuda", generator=gen) * 2
+    tokens = torch.randint(0, V, (rows,), device="cuda", generator=gen)
+    logits[0, V - 1] = 20.0
+    out = kernel.token_logprobs(logits, tokens, 20)
+    few = logits[:2].contiguous()
+    want, _, _ = reference(few, tokens[:2], 20)
+    assert torch.equal(out.top_tokens[:2].cpu(), want[3])
+    n = units(V)
+    close(out.logprob[:2], want[0], U * (n + 4 * want[0].abs()), "logprob")
+    close(out.top_logprobs[:2], want[2], U * (n + 4 * want[2].abs()), "top_logprobs")
+    close(out.entropy[:2], want[1], U * 3 * n * (1 + math.log(V + 1)), "entropy")
 
 
 def _views(V, dt):
@@ -241,11 +280,11 @@ def test_views(view, dt):
 
 
 def test_a_row_does_not_depend_on_the_others():
-    """Equal bits however many rows come along, as long as the rows are whole workgroups' (512 and more)."""
+    """Equal bits however many rows come along, as long as they take workgroups of one size (2048 rows and more)."""
     say("token_logprobs rows alone")
-    logits, tokens, _ = make(1024, 4001, "bf16", 31)
-    a, b = kernel.token_logprobs(logits, tokens, 4), kernel.token_logprobs(logits[256:], tokens[256:], 4)
-    assert all(torch.equal(s[256:], t) for s, t in zip(a, b))
+    logits, tokens, _ = make(4096, 4001, "bf16", 31)
+    a, b = kernel.token_logprobs(logits, tokens, 4), kernel.token_logprobs(logits[1024:], tokens[1024:], 4)
+    assert all(torch.equal(s[1024:], t) for s, t in zip(a, b))
     c = kernel.token_logprobs(logits, tokens, 4)
     assert all(torch.equal(s, t) for s, t in zip(a, c))
 
@@ -261,12 +300,12 @@ def test_offsets_past_32_bits():
     tokens = torch.randint(0, V, (rows,), generator=gen).cuda()
     x = logits.requires_grad_(True)
     out = kernel.token_logprobs(x, tokens, 2)
-    few = kernel.token_logprobs(last.repeat(300, 1), tokens[-2:].repeat(300), 2)   # whole rows here as well
+    few = kernel.token_logprobs(last.repeat(1050, 1), tokens[-2:].repeat(1050), 2)   # workgroups of the same size
     assert all(torch.equal(a[-2:], b[:2]) for a, b in zip(out, few))
     assert (out.logprob[:-2] + math.log(V)).abs().max() <= U * (units(V) + 44)
     g, = torch.autograd.grad(out.logprob.sum(), x)
     y = last.clone().requires_grad_(True)
-    h, = torch.autograd.grad(kernel.token_logprobs(y.repeat(300, 1), tokens[-2:].repeat(300), 2).logprob[:2].sum(), y)
+    h, = torch.autograd.grad(kernel.token_logprobs(y.repeat(1050, 1), tokens[-2:].repeat(1050), 2).logprob[:2].sum(), y)
     assert torch.equal(g[-2:], h)
 
 

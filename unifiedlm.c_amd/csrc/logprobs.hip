@@ -16,13 +16,17 @@
 namespace ulm {
 namespace lp {
 
-constexpr int kThreads = 256;
 constexpr int kUnroll = 4;            // 16-byte loads in flight per thread
 constexpr int kMaxTop = 64;           // one lane of a wave each
-constexpr int kMaxParts = 16;
+constexpr int kMaxParts = 64;
+constexpr int kTable = 4096;          // maxima of a workgroup's batches kept for the alternatives
+constexpr int kHits = 512;            // batches read again at once
 constexpr int kCap = 1024;            // candidates held at once
+constexpr int kTies = 512 + kMaxTop;  // and equal ones, taken 512 at a time
 constexpr float kLog2e = 1.44269504088896341f;
-constexpr float kFloor = -1e4f;       // e^d is 0 from here on: keeps 0 x (-inf) out of the sums
+constexpr float kLn2 = 0.693147180559945309f;
+constexpr float kFloor = -1e4f;       // 2^t and e^d are 0 from here on: keeps 0 x (-inf) out of the sums
+constexpr float kHuge = 0x1p96f;      // maxima beyond which m log2(e) is not formed
 
 typedef uint32_t u32x4_any __attribute__((vector_size(16), aligned(2)));   // rows may start anywhere
 
@@ -78,6 +82,13 @@ __device__ __forceinline__ float value_of(uint64_t key) {
 
 __device__ __forceinline__ float exp_of(float d) { return __builtin_amdgcn_exp2f(d * kLog2e); }
 
+// The larger one of numbers; three at a time, and without the quieting of a signalling NaN that fmaxf adds
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float r;
+    asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+    return r;
+}
+
 // The sums of a set of logits about their maximum m: s = sum e^(x - m), u = sum e^(x - m) (x - m).
 struct Sums {
     float m, s, u;
@@ -97,22 +108,36 @@ struct Sums {
 };
 
 __device__ __forceinline__ Sums wave_add(Sums v) {
+    float to = v.m;
 #pragma unroll
-    for (int off = 32; off > 0; off >>= 1) {
-        Sums o;
-        o.m = __shfl_xor(v.m, off, kWave);
-        o.s = __shfl_xor(v.s, off, kWave);
-        o.u = __shfl_xor(v.u, off, kWave);
-        // the same operations in the same order on both lanes: both end with the same bits
-        if (threadIdx.x & off) {
-            o.add(v);
-            v = o;
-        } else {
-            v.add(o);
-        }
-    }
+    for (int off = 32; off > 0; off >>= 1) to = fmaxf(to, __shfl_xor(to, off, kWave));
+    v.rebase(to);
+    v.s = wave_sum(v.s);
+    v.u = wave_sum(v.u);
     return v;
 }
+
+// A thread's running sums in powers of two about ref = m log2(e), rounded: s = sum 2^t_i,
+// u = sum 2^t_i t_i with t_i = x_i log2(e) - ref in one fused operation (6 instructions an
+// element, conversion and maximum included, where differences from m itself take 8). What ref
+// lacks of m log2(e) is put right at the end. Where |m| is so large that ref could
+// overflow (rows masked with the type's lowest value), t_i = (x_i - m) log2(e).
+struct Running {
+    float m = -INFINITY, s = 0.f, u = 0.f;
+    static __device__ __forceinline__ float ref(float m) { return m * kLog2e; }
+    __device__ __forceinline__ bool plain() const { return fabsf(m) < kHuge; }
+    __device__ __forceinline__ void rebase(float to) {   // to > m
+        const float d = plain() && fabsf(to) < kHuge ? ref(m) - ref(to) : (m - to) * kLog2e;
+        const float t = fmaxf(d, kFloor), f = __builtin_amdgcn_exp2f(t);   // m = -inf: s and u are 0
+        u = f * __builtin_fmaf(s, t, u);
+        s *= f;
+        m = to;
+    }
+    __device__ __forceinline__ Sums sums() const {
+        const float lacks = plain() ? __builtin_fmaf(m, kLog2e, -ref(m)) : 0.f, f = __builtin_amdgcn_exp2f(-lacks);
+        return {m, s * f, kLn2 * f * __builtin_fmaf(-lacks, s, u)};
+    }
+};
 
 // Workgroup b of n: the grid's second dimension takes what the first cannot count.
 constexpr long long kGridX = 1 << 20;
@@ -165,171 +190,227 @@ __device__ __forceinline__ void put_top(const Rows &a, const Outs &o, long long 
     o.top_tokens[r * a.top + rank] = index_of(key);
 }
 
-// The `top` largest of elements [e0, e1), as keys in `list`, and how many of the list's
-// entries there are (at least `top` where there are as many elements).
+// The workgroup's batches: batch k of a thread is its kUnroll vectors of tile k.
+template <int DT, int NT> struct Tile {
+    static constexpr int vec = Elem<DT>::vec, size = NT * vec * kUnroll, batches = kTable / NT;
+    static __device__ __forceinline__ int at(int e0, int k, int j, int tid) { return e0 + k * size + (j * NT + tid) * vec; }
+};
+
+struct TopScratch {
+    uint64_t list[kCap + kTies];
+    float table[kTable];
+    int hits[kHits];
+    int rank[kWave];
+    int count, hit_count;
+    uint64_t bound;
+};
+
+// The keys of elements [e0, e1) among which the `top` largest are, in sc.list; returns their number.
 //
-// Every thread knows its own largest element; the top-th largest of 64 groups' maxima is
-// no more than the top-th largest element of all, and whatever is no less than it lies in
-// the at most `top` groups whose maximum is. Those threads read their elements again.
-// Should more than kCap elements pass, the top-th largest of the kCap that were kept is a
-// higher such bound, and all but `top` of those kCap fall below it: every turn leaves out
-// kCap - top elements or more.
-template <int DT>
-__device__ int candidates(const char *row, int e0, int e1, int top, uint64_t mine, bool all, uint64_t *list,
-                          uint64_t *groups, int *count, uint64_t *bound) {
-    constexpr int V = Elem<DT>::vec;
-    const int tid = threadIdx.x, lane = tid % kWave;
-    groups[tid] = mine;
-    if (tid == 0) *count = 0;
+// sc.table holds every thread's largest element of each batch (NaN where the batch has one) and
+// `mine` is the thread's largest of all. The top-th largest of 64 groups' maxima (a lane's
+// across the waves), `low`, is no more than the top-th largest element; the few batches
+// whose maximum is no less are read again, all of them at once. Where that is too many for
+// the lists:
+//   - many elements equal to `low` (a masked row, say): those above it, and in the order
+//     of the row as many equal ones as are wanted;
+//   - many above it (they lie in a few groups): every element is looked at in turns, each
+//     with a higher bound, the top-th largest of the kCap keys that the turn before kept, so
+//     that a turn leaves out kCap - top elements or more.
+template <int DT, int NT>
+__device__ int candidates(const char *row, int e0, int e1, int top, float mine, TopScratch &sc) {
+    using T = Tile<DT, NT>;
+    constexpr int V = T::vec, W = NT / kWave;
+    static_assert(W <= kWave && kWave % W == 0, "a share of the groups for every wave");
+    const int tid = threadIdx.x, lane = tid % kWave, wave = tid / kWave;
+    const int batches = (e1 - e0 + T::size - 1) / T::size;
+    float *maxima = reinterpret_cast<float *>(sc.list);   // not in use yet
+    static_assert(NT * sizeof(float) <= sizeof(sc.list), "scratch");
+    maxima[tid] = mine;
+    if (tid < kWave) sc.rank[tid] = 0;
     __syncthreads();
-    if (tid < kWave) {
-        uint64_t k = groups[lane];
+    float group = maxima[lane];
 #pragma unroll
-        for (int w = 1; w < kThreads / kWave; ++w) {
-            const uint64_t o = groups[lane + w * kWave];
-            k = o > k ? o : k;
-        }
-        int rank = 0;
-        for (int j = 0; j < kWave; ++j) {
-            const uint64_t o = __shfl(k, j, kWave);
-            rank += o > k || (o == k && j < lane);   // empty groups share the key 0
-        }
-        if (rank == top - 1) *bound = k;
+    for (int w = 1; w < W; ++w) group = fmaxf(group, maxima[lane + w * kWave]);
+    int rank = 0;
+#pragma unroll
+    for (int i = 0; i < kWave / W; ++i) {
+        const int j = wave * (kWave / W) + i;
+        const float o = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(group), j));
+        rank += o > group || (o == group && j < lane);
     }
+    atomicAdd(&sc.rank[lane], rank);
+    if (tid == 0) sc.count = sc.hit_count = 0;
     __syncthreads();
-    for (;;) {
-        const uint64_t low = *bound;
-        if (all || mine >= low) {
-            for (int i = e0 + tid * V; i < e1; i += kThreads * V) {
-                float x[V];
-                load_vec<DT>(row, i, e1, x);
+    const uint64_t which = __ballot(sc.rank[lane] == top - 1);   // one lane
+    const float low = __shfl(group, __ffsll(static_cast<unsigned long long>(which)) - 1, kWave);
+
+    auto push = [&](uint64_t key) {
+        const int at = atomicAdd(&sc.count, 1);
+        if (at < kCap + kTies) sc.list[at] = key;
+    };
+    auto gather = [&](auto wanted) {   // the wanted elements, or more than kCap; counts are 0 before
+        for (int k = 0; k < batches; ++k)
+            if (wanted(sc.table[k * NT + tid])) {
+                const int at = atomicAdd(&sc.hit_count, 1);
+                if (at < kHits) sc.hits[at] = k * NT + tid;
+            }
+        __syncthreads();
+        const int hits = sc.hit_count;
+        if (hits > kHits) return kCap + 1;
+        for (int h = tid / kUnroll; h < hits; h += NT / kUnroll) {
+            const int i = T::at(e0, sc.hits[h] / NT, tid % kUnroll, sc.hits[h] % NT);
+            if (i >= e1) continue;
+            float x[V];
+            load_vec<DT>(row, i, e1, x);
 #pragma unroll
-                for (int k = 0; k < V; ++k) {
-                    const uint64_t key = key_of(x[k], i + k);
-                    if (i + k < e1 && key >= low) {
-                        const int at = atomicAdd(count, 1);
-                        if (at < kCap) list[at] = key;
-                    }
+            for (int k = 0; k < V; ++k)
+                if (i + k < e1 && wanted(x[k])) push(key_of(x[k], i + k));
+        }
+        __syncthreads();
+        return sc.count;
+    };
+    int n = gather([low](float x) { return !(x < low); });
+    if (n <= kCap) return n;
+    __syncthreads();
+    if (tid == 0) sc.count = sc.hit_count = 0;
+    __syncthreads();
+    n = gather([low](float x) { return x > low || x != x; });
+    if (n <= kCap) {
+        if (wave == 0) {
+            for (int i = e0 + lane * V; __any(i < e1); i += kWave * V) {
+                if (i < e1) {
+                    float x[V];
+                    load_vec<DT>(row, i, e1, x);
+#pragma unroll
+                    for (int k = 0; k < V; ++k)
+                        if (i + k < e1 && x[k] == low) push(key_of(x[k], i + k));
                 }
+                __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+                __builtin_amdgcn_wave_barrier();
+                if (__builtin_amdgcn_readfirstlane(*const_cast<volatile int *>(&sc.count)) >= n + top) break;
             }
         }
         __syncthreads();
-        const int n = *count;
-        if (n <= kCap) return n;
+        return sc.count;
+    }
+    if (tid == 0) sc.bound = 0;   // every key
+    for (;;) {
         __syncthreads();
-        if (tid == 0) *count = 0;
-        for (int i = tid; i < kCap; i += kThreads) {
-            const uint64_t k = list[i];
-            int rank = 0;
-            for (int j = 0; j < kCap; ++j) rank += list[j] > k;
-            if (rank == top - 1) *bound = k;
+        if (tid == 0) sc.count = 0;
+        __syncthreads();
+        const uint64_t bound = sc.bound;
+        for (int i = e0 + tid * V; i < e1; i += NT * V) {
+            float x[V];
+            load_vec<DT>(row, i, e1, x);
+#pragma unroll
+            for (int k = 0; k < V; ++k) {
+                const uint64_t key = key_of(x[k], i + k);
+                if (i + k < e1 && !(x[k] < low) && key >= bound) push(key);
+            }
         }
         __syncthreads();
+        n = sc.count;
+        if (n <= kCap) return n;
+        for (int i = tid; i < kCap; i += NT) {
+            const uint64_t k = sc.list[i];
+            int above = 0;
+            for (int j = 0; j < kCap; ++j) above += sc.list[j] > k;
+            if (above == top - 1) sc.bound = k;
+        }
     }
 }
 
-// One workgroup per (row, part). With one part it writes the row's outputs, with more the
-// part's sums and its `top` best keys in order (0 where it has fewer).
-template <int DT, bool TOP>
-__global__ __launch_bounds__(kThreads) void fwd_kernel(Rows a, Outs o, Sums *part_sums, uint64_t *part_keys) {
-    constexpr int V = Elem<DT>::vec, kTile = kThreads * V * kUnroll;
+// One workgroup of NT threads per (row, part). With one part it writes the row's outputs, with
+// more the part's sums and its `top` best keys in order (0 where it has fewer).
+template <int DT, bool TOP, int NT>
+__global__ __launch_bounds__(NT) void fwd_kernel(Rows a, Outs o, Sums *part_sums, uint64_t *part_keys) {
+    using T = Tile<DT, NT>;
+    constexpr int V = T::vec;
     const long long id = block_id(), r = id / a.parts;
     if (r >= a.rows) return;
     const int tid = threadIdx.x, part = static_cast<int>(id % a.parts);
     const char *row = a.row(r, Elem<DT>::bytes);
     const int e0 = part * a.part_len, e1 = min(a.V, e0 + a.part_len);
+    __shared__ std::conditional_t<TOP, TopScratch, int> scratch;
 
-    Sums v{-INFINITY, 0.f, 0.f};
-    float best = -INFINITY;
-    int best_at = e0;   // the tile that holds the thread's first largest element
-    for (int t = e0; t < e1; t += kTile) {
+    Running v;
+    for (int k = 0; e0 + k * T::size < e1; ++k) {
         float x[kUnroll][V];
-        if (t + kTile <= e1) {
+        if (e0 + (k + 1) * T::size <= e1) {
             u32x4_any w[kUnroll];
 #pragma unroll
             for (int j = 0; j < kUnroll; ++j)
-                w[j] = *reinterpret_cast<const u32x4_any *>(row + static_cast<size_t>(t + (j * kThreads + tid) * V) * Elem<DT>::bytes);
+                w[j] = *reinterpret_cast<const u32x4_any *>(row + static_cast<size_t>(T::at(e0, k, j, tid)) * Elem<DT>::bytes);
 #pragma unroll
             for (int j = 0; j < kUnroll; ++j) unpack<DT>(w[j], x[j]);
         } else {
 #pragma unroll
-            for (int j = 0; j < kUnroll; ++j) load_vec<DT>(row, t + (j * kThreads + tid) * V, e1, x[j]);
+            for (int j = 0; j < kUnroll; ++j) load_vec<DT>(row, T::at(e0, k, j, tid), e1, x[j]);
         }
-        float most = x[0][0];
+        float most = -INFINITY;
 #pragma unroll
         for (int j = 0; j < kUnroll; ++j)
 #pragma unroll
-            for (int k = 0; k < V; ++k) most = fmaxf(most, x[j][k]);
-        if (TOP && most > best) {
-            best = most;
-            best_at = t;
-        }
+            for (int i = 0; i < V; i += 2) most = max3(most, x[j][i], x[j][i + 1]);
         if (most > v.m) v.rebase(most);
-        if (v.m == -INFINITY) {   // nothing but masked elements so far (or NaN)
+            if (v.m == -INFINITY) {   // nothing but masked elements so far (or NaN)
 #pragma unroll
             for (int j = 0; j < kUnroll; ++j)
 #pragma unroll
-                for (int k = 0; k < V; ++k) v.s += x[j][k] != x[j][k] ? x[j][k] : 0.f;
-            continue;
+                for (int i = 0; i < V; ++i) v.s += x[j][i] != x[j][i] ? x[j][i] : 0.f;
+        } else if (v.plain()) {
+            const float ref = -Running::ref(v.m);
+#pragma unroll
+            for (int j = 0; j < kUnroll; ++j)
+#pragma unroll
+                for (int i = 0; i < V; ++i) {
+                    const float t = __builtin_fmaf(x[j][i], kLog2e, ref), e = __builtin_amdgcn_exp2f(t);
+                    v.s += e;
+                    v.u = __builtin_fmaf(e, fmaxf(t, kFloor), v.u);
+                }
+        } else {
+#pragma unroll
+            for (int j = 0; j < kUnroll; ++j)
+#pragma unroll
+                for (int i = 0; i < V; ++i) {
+                    const float t = (x[j][i] - v.m) * kLog2e, e = __builtin_amdgcn_exp2f(t);
+                    v.s += e;
+                    v.u = __builtin_fmaf(e, fmaxf(t, kFloor), v.u);
+                }
         }
-#pragma unroll
-        for (int j = 0; j < kUnroll; ++j)
-#pragma unroll
-            for (int k = 0; k < V; ++k) {
-                const float d = x[j][k] - v.m, e = exp_of(d);
-                v.s += e;
-                v.u = __builtin_fmaf(e, fmaxf(d, kFloor), v.u);
-            }
+        if constexpr (TOP) scratch.table[k * NT + tid] = v.s == v.s ? most : __uint_as_float(0x7fc00000u);
     }
 
-    __shared__ Sums waves[kThreads / kWave];
-    const bool odd = v.s != v.s;   // a NaN among the thread's elements
-    const Sums w = wave_add(v);
+    __shared__ Sums waves[NT / kWave];
+    __shared__ float ml[2];
+    const Sums w = wave_add(v.sums());
     if (tid % kWave == 0) waves[tid / kWave] = w;
     __syncthreads();
-    Sums all = waves[0];
-#pragma unroll
-    for (int k = 1; k < kThreads / kWave; ++k) all.add(waves[k]);
-
-    float m = 0.f, logs = 0.f;
-    __shared__ float ml[2];
     if (tid == 0) {
-        if (a.parts == 1) {
-            finish_row<DT>(a, o, r, all, m, logs);
-            ml[0] = m;
-            ml[1] = logs;
-        } else {
-            part_sums[id] = all;
-        }
+        Sums all = waves[0];
+#pragma unroll
+        for (int k = 1; k < NT / kWave; ++k) all.add(waves[k]);
+        if (a.parts == 1) finish_row<DT>(a, o, r, all, ml[0], ml[1]);
+        else part_sums[id] = all;
     }
     if constexpr (TOP) {
-        __shared__ uint64_t list[kCap], groups[kThreads], bound;
-        __shared__ int count;
-        uint64_t mine = 0;   // the key of the thread's largest element that is no NaN
-        for (int j = kUnroll - 1; j >= 0; --j) {
-            const int i = best_at + (j * kThreads + tid) * V;
-            if (i >= e1) continue;
-            float x[V];
-            load_vec<DT>(row, i, e1, x);
-#pragma unroll
-            for (int k = V - 1; k >= 0; --k)
-                if (i + k < e1 && x[k] == best) mine = key_of(x[k], i + k);
-        }
-        const int n = candidates<DT>(row, e0, e1, a.top, mine, odd, list, groups, &count, &bound);
-        m = ml[0];
-        logs = ml[1];
-        for (int i = tid; i < n; i += kThreads) {
-            const uint64_t k = list[i];
+        const int n = candidates<DT, NT>(row, e0, e1, a.top, v.m, scratch);
+        const float m = ml[0], logs = ml[1];
+        for (int i = tid; i < n; i += NT) {
+            const uint64_t k = scratch.list[i];
             int rank = 0;
-            for (int j = 0; j < n; ++j) rank += list[j] > k;
+            for (int j = 0; j < n; ++j) rank += scratch.list[j] > k;
             if (rank >= a.top) continue;
             if (a.parts == 1) put_top(a, o, r, rank, k, m, logs);
             else part_keys[id * a.top + rank] = k;
         }
         if (a.parts > 1)
-            for (int i = n + tid; i < a.top; i += kThreads) part_keys[id * a.top + i] = 0;
+            for (int i = n + tid; i < a.top; i += NT) part_keys[id * a.top + i] = 0;
     }
 }
+
+constexpr int kThreads = 256;   // of the kernels below
 
 // The parts of a row joined: one workgroup per row.
 template <int DT, bool TOP>
@@ -337,7 +418,7 @@ __global__ __launch_bounds__(kThreads) void join_kernel(Rows a, Outs o, const Su
     const long long r = blockIdx.x;
     const int tid = threadIdx.x;
     __shared__ float ml[2];
-    __shared__ uint64_t list[kMaxParts * kMaxTop];
+    __shared__ uint64_t list[TOP ? kMaxParts * kMaxTop : 1];
     const int n = TOP ? a.parts * a.top : 0;
     for (int i = tid; i < n; i += kThreads) list[i] = part_keys[r * n + i];
     if (tid == 0) {
@@ -423,14 +504,20 @@ __global__ __launch_bounds__(kThreads) void bwd_kernel(Rows a, Grads g, int tile
     }
 }
 
-// Parts a row is split into: a function of the sizes, the same for the workspace and the launch.
-inline int parts_of(long long rows, int V) {
-    if (rows >= 512) return 1;
-    long long p = (1024 + rows - 1) / rows;
-    const long long most = (V + 2047) / 2048;
-    if (p > most) p = most;
-    if (p > kMaxParts) p = kMaxParts;
-    return p < 1 ? 1 : static_cast<int>(p);
+// How the rows are spread: a function of the sizes, the same for the workspace and the launch.
+struct Plan {
+    int threads, parts, part_len;
+};
+inline Plan plan_of(long long rows, int V, int top) {
+    Plan p{rows >= 2048 ? 256 : 1024, 1, V};
+    // the alternatives' table holds kTable batches of at least 4 kUnroll elements
+    const long long most = static_cast<long long>(kTable) * kUnroll * 4;
+    long long parts = top ? (V + most - 1) / most : 1;
+    if (parts > 1) {
+        p.parts = static_cast<int>(parts);
+        p.part_len = static_cast<int>((V + parts * 8 - 1) / (parts * 8) * 8);   // whole 8-element vectors
+    }
+    return p;
 }
 
 }  // namespace lp
@@ -442,6 +529,7 @@ static int check_rows(const char *fn, long long rows, long long inner, int V, in
     if (rows < 1 || rows > (1LL << 34) || inner < 1 || V < 1 || V > (1 << 30))
         return fail(ULM_ERR_INVALID, "%s: bad sizes rows=%lld inner=%lld V=%d", fn, rows, inner, V);
     if (top < 0 || top > lp::kMaxTop || top > V) return fail(ULM_ERR_INVALID, "%s: top=%d outside 0 .. min(V, %d)", fn, top, lp::kMaxTop);
+    if (top && V > lp::kMaxParts * lp::kTable * lp::kUnroll * 4) return fail(ULM_ERR_INVALID, "%s: top=%d with V=%d", fn, top, V);
     if (!valid_dtype(dtype)) return fail(ULM_ERR_INVALID, "%s: bad dtype %d", fn, dtype);
     return ULM_OK;
 }
@@ -450,7 +538,7 @@ extern "C" int ulm_token_logprobs_max_top(void) { return lp::kMaxTop; }
 
 extern "C" size_t ulm_token_logprobs_workspace_bytes(long long rows, int V, int top) {
     if (rows < 1 || V < 1 || top < 0 || top > lp::kMaxTop) return 0;
-    const int parts = lp::parts_of(rows, V);
+    const int parts = lp::plan_of(rows, V, top).parts;
     if (parts == 1) return 0;
     Carver c(nullptr);
     c.take<lp::Sums>(static_cast<size_t>(rows) * parts);
@@ -465,21 +553,21 @@ extern "C" int ulm_token_logprobs(const void *logits, int dtype, const long long
     ULM_TRY(check_rows("ulm_token_logprobs", rows, inner, V, top, dtype));
     ULM_REQUIRE(logits && tokens && logprob && entropy && (top == 0 || (top_logprobs && top_tokens)),
                 "ulm_token_logprobs: null pointer");
-    const int parts = lp::parts_of(rows, V);
+    const lp::Plan plan = lp::plan_of(rows, V, top);
+    const int parts = plan.parts;
     const size_t need = ulm_token_logprobs_workspace_bytes(rows, V, top);
     ULM_REQUIRE(workspace_bytes >= need && (need == 0 || workspace), "ulm_token_logprobs: workspace %zu < %zu", workspace_bytes, need);
     Carver c(workspace);
     lp::Sums *sums = parts > 1 ? c.take<lp::Sums>(static_cast<size_t>(rows) * parts) : nullptr;
     uint64_t *keys = parts > 1 ? c.take<uint64_t>(static_cast<size_t>(rows) * parts * top) : nullptr;
-    // parts of whole 8-element vectors
-    const int part_len = parts == 1 ? V : (V + parts * 8 - 1) / (parts * 8) * 8;
-    const lp::Rows a{static_cast<const char *>(logits), tokens, inner, outer_stride, row_stride, ignore_index, rows, V, top, parts, part_len};
+    const lp::Rows a{static_cast<const char *>(logits), tokens, inner, outer_stride, row_stride, ignore_index, rows, V, top, parts, plan.part_len};
     const lp::Outs o{logprob, entropy, top_logprobs, stats, top_tokens};
     hipStream_t s = static_cast<hipStream_t>(stream);
     auto launch = [&](auto dt, auto with_top) {
         constexpr int DT = decltype(dt)::value;
         constexpr bool TOP = decltype(with_top)::value;
-        lp::fwd_kernel<DT, TOP><<<lp::grid_of(rows * parts), dim3(lp::kThreads), 0, s>>>(a, o, sums, keys);
+        if (plan.threads == 256) lp::fwd_kernel<DT, TOP, 256><<<lp::grid_of(rows * parts), dim3(256), 0, s>>>(a, o, sums, keys);
+        else lp::fwd_kernel<DT, TOP, 1024><<<lp::grid_of(rows * parts), dim3(1024), 0, s>>>(a, o, sums, keys);
         if (parts > 1)
             lp::join_kernel<DT, TOP><<<lp::grid_of(rows), dim3(lp::kThreads), 0, s>>>(a, o, sums, keys);
     };
