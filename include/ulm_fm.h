@@ -409,7 +409,7 @@ int ulm_decode_step(const ulm_decode_layer *layers, int n_layers, const float *x
  * gradients of logprob (rows,), entropy (rows,) and top_logprobs (rows, top), each fp32 or NULL:
  *   dx_i = a [i = t] + sum_j c_j [i = top_j] - p_i (a + sum_j c_j + h (ln p_i + entropy)). */
 int ulm_token_logprobs_max_top(void);
-size_t ulm_token_logprobs_workspace_bytes(long long rows, int V, int top);
+size_t ulm_token_logprobs_workspace_bytes(long long rows, int V, int top, int dtype);
 int ulm_token_logprobs(const void *logits, int dtype, const long long *tokens, long long rows, long long inner,
                        long long outer_stride, long long row_stride, int V, int top, long long ignore_index,
                        float *logprob, float *entropy, float *top_logprobs, long long *top_tokens, float *stats,

@@ -280,7 +280,7 @@ def test_views(view, dt):
 
 
 def test_a_row_does_not_depend_on_the_others():
-    """Equal bits however many rows come along, as long as they take workgroups of one size (2048 rows and more)."""
+    """Equal bits however many rows come along, as long as they take workgroups of one size (more than 512 rows)."""
     say("token_logprobs rows alone")
     logits, tokens, _ = make(4096, 4001, "bf16", 31)
     a, b = kernel.token_logprobs(logits, tokens, 4), kernel.token_logprobs(logits[1024:], tokens[1024:], 4)

@@ -601,7 +601,7 @@ struct TokenLogprobs : torch::autograd::Function<TokenLogprobs> {
             *stats = make(with);
         }
         if (r.rows) {
-            const size_t wb = ulm_token_logprobs_workspace_bytes(r.rows, r.V, top);
+            const size_t wb = ulm_token_logprobs_workspace_bytes(r.rows, r.V, top, code(logits.scalar_type()));
             const Tensor ws = wb ? make.bytes(wb) : Tensor();
             check("ulm_token_logprobs",
                   ulm_token_logprobs(r.x.data_ptr(), code(logits.scalar_type()), ip(tok), r.rows, r.inner, r.outer_stride,

@@ -18,17 +18,17 @@ namespace lp {
 
 constexpr int kUnroll = 4;            // 16-byte loads in flight per thread
 constexpr int kMaxTop = 64;           // one lane of a wave each
-constexpr int kMaxParts = 64;
-constexpr int kTable = 4096;          // maxima of a workgroup's batches kept for the alternatives
-constexpr int kHits = 512;            // batches read again at once
-constexpr int kCap = 1024;            // candidates held at once
-constexpr int kTies = 512 + kMaxTop;  // and equal ones, taken 512 at a time
+constexpr int kMaxParts = 64;          // a row's, one lane of a wave each
+constexpr int kMaxTopV = 1 << 22;      // columns with alternatives: kMaxParts parts of 65536
 constexpr float kLog2e = 1.44269504088896341f;
 constexpr float kLn2 = 0.693147180559945309f;
 constexpr float kFloor = -1e4f;       // 2^t and e^d are 0 from here on: keeps 0 x (-inf) out of the sums
 constexpr float kHuge = 0x1p96f;      // maxima beyond which m log2(e) is not formed
 
 typedef uint32_t u32x4_any __attribute__((vector_size(16), aligned(2)));   // rows may start anywhere
+
+// 16 bytes of a stream that the caches need not keep (bf16 rows of 32000: 6.7 TB/s, 5.9 with ordinary loads)
+__device__ __forceinline__ u32x4_any load_once(const char *p) { return __builtin_nontemporal_load(reinterpret_cast<const u32x4_any *>(p)); }
 
 template <int DT> struct Elem { static constexpr int vec = DT == ULM_F32 ? 4 : 8, bytes = DT == ULM_F32 ? 4 : 2; };
 
@@ -61,7 +61,7 @@ template <int DT>
 __device__ __forceinline__ void load_vec(const char *row, int i, int end, float (&x)[Elem<DT>::vec]) {
     constexpr int V = Elem<DT>::vec;
     if (i + V <= end) {
-        unpack<DT>(*reinterpret_cast<const u32x4_any *>(row + static_cast<size_t>(i) * Elem<DT>::bytes), x);
+        unpack<DT>(load_once(row + static_cast<size_t>(i) * Elem<DT>::bytes), x);
     } else {
 #pragma unroll
         for (int k = 0; k < V; ++k) x[k] = i + k < end ? load_as_f32(row, i + k, DT) : -INFINITY;
@@ -98,22 +98,19 @@ struct Sums {
         s *= f;
         m = to;
     }
-    __device__ __forceinline__ void add(Sums o) {
-        const float to = fmaxf(m, o.m);
-        rebase(to);
-        o.rebase(to);
-        s += o.s;
-        u += o.u;
-    }
 };
 
-__device__ __forceinline__ Sums wave_add(Sums v) {
+// over groups of W lanes
+template <int W> __device__ __forceinline__ Sums group_add(Sums v) {
     float to = v.m;
 #pragma unroll
-    for (int off = 32; off > 0; off >>= 1) to = fmaxf(to, __shfl_xor(to, off, kWave));
+    for (int off = W / 2; off > 0; off >>= 1) to = fmaxf(to, __shfl_xor(to, off, kWave));
     v.rebase(to);
-    v.s = wave_sum(v.s);
-    v.u = wave_sum(v.u);
+#pragma unroll
+    for (int off = W / 2; off > 0; off >>= 1) {
+        v.s += __shfl_xor(v.s, off, kWave);
+        v.u += __shfl_xor(v.u, off, kWave);
+    }
     return v;
 }
 
@@ -153,7 +150,8 @@ struct Rows {
     long long ignore, rows;
     int V, top, parts, part_len;
     __device__ __forceinline__ const char *row(long long r, int bytes) const {
-        return x + ((r / inner) * outer_stride + (r % inner) * row_stride) * bytes;
+        const long long outer = outer_stride ? r / inner : 0;
+        return x + (outer * outer_stride + (r - outer * inner) * row_stride) * bytes;
     }
 };
 
@@ -162,19 +160,23 @@ struct Outs {
     long long *top_tokens;
 };
 
-// what every row ends with, on one thread: its log probability, entropy and (m, ln s)
-template <int DT>
-__device__ __forceinline__ void finish_row(const Rows &a, const Outs &o, long long r, Sums v, float &m, float &logs) {
+// what every row ends with, on one thread: its log probability, entropy and (m, ln s). The token t and,
+// where there is one, its logit x were read ahead.
+struct Target {
+    long long t;
+    float x;
+};
+template <int DT> __device__ __forceinline__ Target target_of(const Rows &a, const char *row, long long r) {
+    const long long t = a.tokens[r];
+    return {t, t >= 0 && t < a.V ? load_as_f32(row, t, DT) : 0.f};
+}
+__device__ __forceinline__ void finish_row(const Rows &a, const Outs &o, long long r, Target to, Sums v, float &m, float &logs) {
     logs = v.s > 0.f ? logf(v.s) : v.s == 0.f ? -INFINITY : v.s;   // an empty row: -inf; a NaN stays
     m = v.m;
-    const long long t = a.tokens[r];
     float lp = 0.f;
-    if (t != a.ignore) {
+    if (to.t != a.ignore) {
         lp = __uint_as_float(0x7fc00000u);
-        if (t >= 0 && t < a.V) {
-            const float x = load_as_f32(a.row(r, Elem<DT>::bytes), t, DT);
-            lp = v.s == 0.f ? -INFINITY : (x - m) - logs;
-        }
+        if (to.t >= 0 && to.t < a.V) lp = v.s == 0.f ? -INFINITY : (to.x - m) - logs;
     }
     o.logprob[r] = lp;
     o.entropy[r] = v.s == 0.f ? 0.f : logs - v.u / v.s;
@@ -192,14 +194,19 @@ __device__ __forceinline__ void put_top(const Rows &a, const Outs &o, long long 
 
 // The workgroup's batches: batch k of a thread is its kUnroll vectors of tile k.
 template <int DT, int NT> struct Tile {
-    static constexpr int vec = Elem<DT>::vec, size = NT * vec * kUnroll, batches = kTable / NT;
+    static constexpr int vec = Elem<DT>::vec, size = NT * vec * kUnroll;
     static __device__ __forceinline__ int at(int e0, int k, int j, int tid) { return e0 + k * size + (j * NT + tid) * vec; }
 };
 
-struct TopScratch {
-    uint64_t list[kCap + kTies];
-    float table[kTable];
-    int hits[kHits];
+// Room for the alternatives of a unit, by the workgroup's size, so that small ones fill a CU.
+constexpr int batches_of(int NT) { return NT <= 256 ? 16 : 8; }
+template <int NT> struct TopScratch {
+    static constexpr int cap = NT < 256 ? 4 * NT : 1024;     // candidates held at once
+    static constexpr int most_hits = NT < 256 ? 2 * NT : 512;   // batches read again at once
+    static constexpr int tie_lanes = NT < 256 ? 16 : kWave;  // that look for equal ones, 8 elements each
+    uint64_t list[cap + 8 * tie_lanes + kMaxTop];
+    float table[batches_of(NT) * NT];   // the batches' maxima
+    int hits[most_hits];
     int rank[kWave];
     int count, hit_count;
     uint64_t bound;
@@ -218,9 +225,10 @@ struct TopScratch {
 //     with a higher bound, the top-th largest of the kCap keys that the turn before kept, so
 //     that a turn leaves out kCap - top elements or more.
 template <int DT, int NT>
-__device__ int candidates(const char *row, int e0, int e1, int top, float mine, TopScratch &sc) {
+__device__ int candidates(const char *row, int e0, int e1, int top, float mine, TopScratch<NT> &sc) {
     using T = Tile<DT, NT>;
-    constexpr int V = T::vec, W = NT / kWave;
+    constexpr int V = T::vec, W = NT / kWave, kCap = TopScratch<NT>::cap, kHits = TopScratch<NT>::most_hits;
+    constexpr int kTieLanes = TopScratch<NT>::tie_lanes;
     static_assert(W <= kWave && kWave % W == 0, "a share of the groups for every wave");
     const int tid = threadIdx.x, lane = tid % kWave, wave = tid / kWave;
     const int batches = (e1 - e0 + T::size - 1) / T::size;
@@ -247,7 +255,7 @@ __device__ int candidates(const char *row, int e0, int e1, int top, float mine, 
 
     auto push = [&](uint64_t key) {
         const int at = atomicAdd(&sc.count, 1);
-        if (at < kCap + kTies) sc.list[at] = key;
+        if (at < static_cast<int>(sizeof(sc.list) / sizeof(key))) sc.list[at] = key;
     };
     auto gather = [&](auto wanted) {   // the wanted elements, or more than kCap; counts are 0 before
         for (int k = 0; k < batches; ++k)
@@ -278,8 +286,8 @@ __device__ int candidates(const char *row, int e0, int e1, int top, float mine, 
     n = gather([low](float x) { return x > low || x != x; });
     if (n <= kCap) {
         if (wave == 0) {
-            for (int i = e0 + lane * V; __any(i < e1); i += kWave * V) {
-                if (i < e1) {
+            for (int i = e0 + lane * V; __any(i < e1); i += kTieLanes * V) {
+                if (i < e1 && lane < kTieLanes) {
                     float x[V];
                     load_vec<DT>(row, i, e1, x);
 #pragma unroll
@@ -321,78 +329,105 @@ __device__ int candidates(const char *row, int e0, int e1, int top, float mine, 
     }
 }
 
+// One batch of a thread added to its running sums; returns the batch's largest element.
+template <int N> __device__ __forceinline__ float take(const float (&x)[N], bool guard, bool &masked, Running &v) {
+    float most = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < N; i += 2) most = max3(most, x[i], x[i + 1]);
+    if (most > v.m) v.rebase(most);
+    if (v.m == -INFINITY) {   // nothing but masked elements so far (or NaN)
+#pragma unroll
+        for (int i = 0; i < N; ++i) v.s += x[i] != x[i] ? x[i] : 0.f;
+    } else if (v.plain()) {
+        const float ref = -Running::ref(v.m);
+        float s = v.s, u = v.u;
+        guard |= masked;
+        if (!guard) {
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                const float t = __builtin_fmaf(x[i], kLog2e, ref), e = __builtin_amdgcn_exp2f(t);
+                s += e;
+                u = __builtin_fmaf(e, t, u);
+            }
+            guard = masked = u != u;   // 0 x (-inf), or a NaN among the elements
+        }
+        if (guard) {
+            s = v.s;
+            u = v.u;
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                const float t = __builtin_fmaf(x[i], kLog2e, ref), e = __builtin_amdgcn_exp2f(t);
+                s += e;
+                u = __builtin_fmaf(e, fmaxf(t, kFloor), u);
+            }
+        }
+        v.s = s;
+        v.u = u;
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const float t = (x[i] - v.m) * kLog2e, e = __builtin_amdgcn_exp2f(t);
+            v.s += e;
+            v.u = __builtin_fmaf(e, fmaxf(t, kFloor), v.u);
+        }
+    }
+    return most;
+}
+
 // One workgroup of NT threads per (row, part). With one part it writes the row's outputs, with
 // more the part's sums and its `top` best keys in order (0 where it has fewer).
 template <int DT, bool TOP, int NT>
 __global__ __launch_bounds__(NT) void fwd_kernel(Rows a, Outs o, Sums *part_sums, uint64_t *part_keys) {
     using T = Tile<DT, NT>;
-    constexpr int V = T::vec;
-    const long long id = block_id(), r = id / a.parts;
+    constexpr int V = T::vec, W = NT / kWave;
+    const long long id = block_id(), r = a.parts == 1 ? id : id / a.parts;
     if (r >= a.rows) return;
-    const int tid = threadIdx.x, part = static_cast<int>(id % a.parts);
+    const int tid = threadIdx.x, part = static_cast<int>(id - r * a.parts);
     const char *row = a.row(r, Elem<DT>::bytes);
     const int e0 = part * a.part_len, e1 = min(a.V, e0 + a.part_len);
-    __shared__ std::conditional_t<TOP, TopScratch, int> scratch;
+    __shared__ std::conditional_t<TOP, TopScratch<NT>, int> scratch;
 
+    const Target to = a.parts == 1 && tid == 0 ? target_of<DT>(a, row, r) : Target{};
     Running v;
+    bool masked = false;   // -inf was met: its t is kept finite from then on
     for (int k = 0; e0 + k * T::size < e1; ++k) {
-        float x[kUnroll][V];
-        if (e0 + (k + 1) * T::size <= e1) {
+        float x[kUnroll * V];
+        const bool whole = e0 + (k + 1) * T::size <= e1;
+        if (e1 - e0 >= V) {   // every load inside the row: the last tile's overhang reads its last elements and drops them
             u32x4_any w[kUnroll];
 #pragma unroll
             for (int j = 0; j < kUnroll; ++j)
-                w[j] = *reinterpret_cast<const u32x4_any *>(row + static_cast<size_t>(T::at(e0, k, j, tid)) * Elem<DT>::bytes);
+                w[j] = load_once(row + static_cast<size_t>(min(T::at(e0, k, j, tid), e1 - V)) * Elem<DT>::bytes);
 #pragma unroll
-            for (int j = 0; j < kUnroll; ++j) unpack<DT>(w[j], x[j]);
+            for (int j = 0; j < kUnroll; ++j) unpack<DT>(w[j], *reinterpret_cast<float(*)[V]>(&x[j * V]));
+            if (!whole) {
+                asm volatile("");   // a branch: 64 selects in every tile otherwise
+#pragma unroll
+                for (int j = 0; j < kUnroll; ++j) {
+                    const int over = T::at(e0, k, j, tid) - (e1 - V);   // the first `over` elements are others'
+#pragma unroll
+                    for (int i = 0; i < V; ++i) x[j * V + i] = i < over ? -INFINITY : x[j * V + i];
+                }
+            }
         } else {
 #pragma unroll
-            for (int j = 0; j < kUnroll; ++j) load_vec<DT>(row, T::at(e0, k, j, tid), e1, x[j]);
+            for (int j = 0; j < kUnroll; ++j) load_vec<DT>(row, T::at(e0, k, j, tid), e1, *reinterpret_cast<float(*)[V]>(&x[j * V]));
         }
-        float most = -INFINITY;
-#pragma unroll
-        for (int j = 0; j < kUnroll; ++j)
-#pragma unroll
-            for (int i = 0; i < V; i += 2) most = max3(most, x[j][i], x[j][i + 1]);
-        if (most > v.m) v.rebase(most);
-            if (v.m == -INFINITY) {   // nothing but masked elements so far (or NaN)
-#pragma unroll
-            for (int j = 0; j < kUnroll; ++j)
-#pragma unroll
-                for (int i = 0; i < V; ++i) v.s += x[j][i] != x[j][i] ? x[j][i] : 0.f;
-        } else if (v.plain()) {
-            const float ref = -Running::ref(v.m);
-#pragma unroll
-            for (int j = 0; j < kUnroll; ++j)
-#pragma unroll
-                for (int i = 0; i < V; ++i) {
-                    const float t = __builtin_fmaf(x[j][i], kLog2e, ref), e = __builtin_amdgcn_exp2f(t);
-                    v.s += e;
-                    v.u = __builtin_fmaf(e, fmaxf(t, kFloor), v.u);
-                }
-        } else {
-#pragma unroll
-            for (int j = 0; j < kUnroll; ++j)
-#pragma unroll
-                for (int i = 0; i < V; ++i) {
-                    const float t = (x[j][i] - v.m) * kLog2e, e = __builtin_amdgcn_exp2f(t);
-                    v.s += e;
-                    v.u = __builtin_fmaf(e, fmaxf(t, kFloor), v.u);
-                }
-        }
+        const float most = take(x, !whole, masked, v);
         if constexpr (TOP) scratch.table[k * NT + tid] = v.s == v.s ? most : __uint_as_float(0x7fc00000u);
     }
 
-    __shared__ Sums waves[NT / kWave];
+    __shared__ Sums waves[W];
     __shared__ float ml[2];
-    const Sums w = wave_add(v.sums());
+    const Sums w = group_add<kWave>(v.sums());
     if (tid % kWave == 0) waves[tid / kWave] = w;
     __syncthreads();
-    if (tid == 0) {
-        Sums all = waves[0];
-#pragma unroll
-        for (int k = 1; k < NT / kWave; ++k) all.add(waves[k]);
-        if (a.parts == 1) finish_row<DT>(a, o, r, all, ml[0], ml[1]);
-        else part_sums[id] = all;
+    if (tid < kWave) {
+        const Sums all = group_add<W>(waves[tid % W]);
+        if (tid == 0) {
+            if (a.parts == 1) finish_row(a, o, r, to, all, ml[0], ml[1]);
+            else part_sums[id] = all;
+        }
     }
     if constexpr (TOP) {
         const int n = candidates<DT, NT>(row, e0, e1, a.top, v.m, scratch);
@@ -421,10 +456,9 @@ __global__ __launch_bounds__(kThreads) void join_kernel(Rows a, Outs o, const Su
     __shared__ uint64_t list[TOP ? kMaxParts * kMaxTop : 1];
     const int n = TOP ? a.parts * a.top : 0;
     for (int i = tid; i < n; i += kThreads) list[i] = part_keys[r * n + i];
-    if (tid == 0) {
-        Sums all = part_sums[r * a.parts];
-        for (int p = 1; p < a.parts; ++p) all.add(part_sums[r * a.parts + p]);
-        finish_row<DT>(a, o, r, all, ml[0], ml[1]);
+    if (tid < kWave) {   // at most a wave's lanes of parts
+        const Sums all = group_add<kWave>(tid < a.parts ? part_sums[r * a.parts + tid] : Sums{-INFINITY, 0.f, 0.f});
+        if (tid == 0) finish_row(a, o, r, target_of<DT>(a, a.row(r, Elem<DT>::bytes), r), all, ml[0], ml[1]);
     }
     if constexpr (TOP) {
         __syncthreads();
@@ -445,15 +479,19 @@ struct Grads {
     char *dx;   // (rows, V), dense
 };
 
-// One workgroup per (row, tile of elements).
+// One workgroup per (row, tile): a vector a thread. At 16384 x 32000 in bf16 338 us, 6.2 TB/s, with
+// stores that leave the caches to others; 404 with ordinary ones, 357 and 360 with two and four
+// vectors a thread.
 template <int DT, bool ENT>
 __global__ __launch_bounds__(kThreads) void bwd_kernel(Rows a, Grads g, int tiles) {
-    constexpr int V = Elem<DT>::vec, kTile = kThreads * V * kUnroll, B = Elem<DT>::bytes;
+    constexpr int V = Elem<DT>::vec, kTile = kThreads * V, B = Elem<DT>::bytes;
     const long long id = block_id(), r = id / tiles;
     if (r >= a.rows) return;
-    const int tid = threadIdx.x, e0 = static_cast<int>(id % tiles) * kTile, e1 = min(a.V, e0 + kTile);
+    const int tid = threadIdx.x, e0 = static_cast<int>(id - r * tiles) * kTile, e1 = min(a.V, e0 + kTile), i = e0 + tid * V;
     const char *row = a.row(r, B);
     char *out = g.dx + static_cast<size_t>(r) * a.V * B;
+    float x[V];
+    if (i < e1) load_vec<DT>(row, i, e1, x);
 
     const float m = g.stats[2 * r], logs = g.stats[2 * r + 1];
     const float h = ENT ? g.dentropy[r] : 0.f, H = ENT ? g.entropy[r] : 0.f;
@@ -469,12 +507,7 @@ __global__ __launch_bounds__(kThreads) void bwd_kernel(Rows a, Grads g, int tile
         const float f = ENT ? __builtin_fmaf(h, (fmaxf(d, kFloor) - logs) + H, G) : G;
         return empty ? 0.f : -p * f;
     };
-#pragma unroll
-    for (int j = 0; j < kUnroll; ++j) {
-        const int i = e0 + (j * kThreads + tid) * V;
-        if (i >= e1) continue;
-        float x[V];
-        load_vec<DT>(row, i, e1, x);
+    if (i < e1) {
         const long long own = t - i;   // the token's place among these
 #pragma unroll
         for (int k = 0; k < V; ++k) {
@@ -488,7 +521,7 @@ __global__ __launch_bounds__(kThreads) void bwd_kernel(Rows a, Grads g, int tile
                 if constexpr (DT == ULM_F32) w[k] = __float_as_uint(x[k]);
                 else w[k] = pack_word<DT>(x[2 * k], x[2 * k + 1]);
             }
-            *reinterpret_cast<u32x4_any *>(out + static_cast<size_t>(i) * B) = w;
+            __builtin_nontemporal_store(w, reinterpret_cast<u32x4_any *>(out + static_cast<size_t>(i) * B));
         } else {
 #pragma unroll
             for (int k = 0; k < V; ++k)
@@ -498,21 +531,28 @@ __global__ __launch_bounds__(kThreads) void bwd_kernel(Rows a, Grads g, int tile
     if (!g.dtop || empty) return;
     __syncthreads();   // the alternatives' elements are written again, with their own terms
     if (tid < a.top) {
-        const long long i = g.top_tokens[r * a.top + tid];
-        if (i >= e0 && i < e1)
-            store_from_f32(out, i, DT, grad(load_as_f32(row, i, DT)) + g.dtop[r * a.top + tid] + (i == t ? da : 0.f));
+        const long long j = g.top_tokens[r * a.top + tid];
+        if (j >= e0 && j < e1)
+            store_from_f32(out, j, DT, grad(load_as_f32(row, j, DT)) + g.dtop[r * a.top + tid] + (j == t ? da : 0.f));
     }
 }
 
-// How the rows are spread: a function of the sizes, the same for the workspace and the launch.
+// How the rows are spread: a function of the sizes, the same for the workspace and the launch. A
+// workgroup as large as leaves a row two tiles, at most 256 threads: at 16384 rows of 200 bf16 16 us
+// with 64 threads (39 with 256); of 8000 48 with 128 (56); of 32000 178 with 256 (183 with 128, 179 with
+// 512; ordinary loads). Up to 512 rows do not fill the device: twice as many threads a row
+// (256 rows of 32000 fp32 and 20 alternatives 10.7 us, 13.1 with 256; one row 7.3 and 9.4).
 struct Plan {
     int threads, parts, part_len;
 };
-inline Plan plan_of(long long rows, int V, int top) {
-    Plan p{rows >= 2048 ? 256 : 1024, 1, V};
-    // the alternatives' table holds kTable batches of at least 4 kUnroll elements
-    const long long most = static_cast<long long>(kTable) * kUnroll * 4;
-    long long parts = top ? (V + most - 1) / most : 1;
+inline Plan plan_of(long long rows, int V, int top, int dtype) {
+    Plan p{64, 1, V};
+    const int vec = dtype == ULM_F32 ? 4 : 8;
+    while (p.threads < 256 && V >= 2 * p.threads * vec * kUnroll) p.threads *= 2;
+    if (rows <= 512 && V >= p.threads * vec * kUnroll / 4) p.threads *= 2;
+    // the alternatives' table holds so many tiles
+    const long long most = static_cast<long long>(batches_of(p.threads)) * p.threads * vec * kUnroll;
+    const long long parts = top ? (V + most - 1) / most : 1;
     if (parts > 1) {
         p.parts = static_cast<int>(parts);
         p.part_len = static_cast<int>((V + parts * 8 - 1) / (parts * 8) * 8);   // whole 8-element vectors
@@ -529,16 +569,16 @@ static int check_rows(const char *fn, long long rows, long long inner, int V, in
     if (rows < 1 || rows > (1LL << 34) || inner < 1 || V < 1 || V > (1 << 30))
         return fail(ULM_ERR_INVALID, "%s: bad sizes rows=%lld inner=%lld V=%d", fn, rows, inner, V);
     if (top < 0 || top > lp::kMaxTop || top > V) return fail(ULM_ERR_INVALID, "%s: top=%d outside 0 .. min(V, %d)", fn, top, lp::kMaxTop);
-    if (top && V > lp::kMaxParts * lp::kTable * lp::kUnroll * 4) return fail(ULM_ERR_INVALID, "%s: top=%d with V=%d", fn, top, V);
+    if (top && V > lp::kMaxTopV) return fail(ULM_ERR_INVALID, "%s: top=%d with V=%d", fn, top, V);
     if (!valid_dtype(dtype)) return fail(ULM_ERR_INVALID, "%s: bad dtype %d", fn, dtype);
     return ULM_OK;
 }
 
 extern "C" int ulm_token_logprobs_max_top(void) { return lp::kMaxTop; }
 
-extern "C" size_t ulm_token_logprobs_workspace_bytes(long long rows, int V, int top) {
-    if (rows < 1 || V < 1 || top < 0 || top > lp::kMaxTop) return 0;
-    const int parts = lp::plan_of(rows, V, top).parts;
+extern "C" size_t ulm_token_logprobs_workspace_bytes(long long rows, int V, int top, int dtype) {
+    if (rows < 1 || V < 1 || top < 0 || top > lp::kMaxTop || !valid_dtype(dtype)) return 0;
+    const int parts = lp::plan_of(rows, V, top, dtype).parts;
     if (parts == 1) return 0;
     Carver c(nullptr);
     c.take<lp::Sums>(static_cast<size_t>(rows) * parts);
@@ -553,9 +593,9 @@ extern "C" int ulm_token_logprobs(const void *logits, int dtype, const long long
     ULM_TRY(check_rows("ulm_token_logprobs", rows, inner, V, top, dtype));
     ULM_REQUIRE(logits && tokens && logprob && entropy && (top == 0 || (top_logprobs && top_tokens)),
                 "ulm_token_logprobs: null pointer");
-    const lp::Plan plan = lp::plan_of(rows, V, top);
+    const lp::Plan plan = lp::plan_of(rows, V, top, dtype);
     const int parts = plan.parts;
-    const size_t need = ulm_token_logprobs_workspace_bytes(rows, V, top);
+    const size_t need = ulm_token_logprobs_workspace_bytes(rows, V, top, dtype);
     ULM_REQUIRE(workspace_bytes >= need && (need == 0 || workspace), "ulm_token_logprobs: workspace %zu < %zu", workspace_bytes, need);
     Carver c(workspace);
     lp::Sums *sums = parts > 1 ? c.take<lp::Sums>(static_cast<size_t>(rows) * parts) : nullptr;
@@ -566,8 +606,11 @@ extern "C" int ulm_token_logprobs(const void *logits, int dtype, const long long
     auto launch = [&](auto dt, auto with_top) {
         constexpr int DT = decltype(dt)::value;
         constexpr bool TOP = decltype(with_top)::value;
-        if (plan.threads == 256) lp::fwd_kernel<DT, TOP, 256><<<lp::grid_of(rows * parts), dim3(256), 0, s>>>(a, o, sums, keys);
-        else lp::fwd_kernel<DT, TOP, 1024><<<lp::grid_of(rows * parts), dim3(1024), 0, s>>>(a, o, sums, keys);
+        const dim3 grid = lp::grid_of(rows * parts);
+        if (plan.threads == 64) lp::fwd_kernel<DT, TOP, 64><<<grid, dim3(64), 0, s>>>(a, o, sums, keys);
+        else if (plan.threads == 128) lp::fwd_kernel<DT, TOP, 128><<<grid, dim3(128), 0, s>>>(a, o, sums, keys);
+        else if (plan.threads == 256) lp::fwd_kernel<DT, TOP, 256><<<grid, dim3(256), 0, s>>>(a, o, sums, keys);
+        else lp::fwd_kernel<DT, TOP, 512><<<grid, dim3(512), 0, s>>>(a, o, sums, keys);
         if (parts > 1)
             lp::join_kernel<DT, TOP><<<lp::grid_of(rows), dim3(lp::kThreads), 0, s>>>(a, o, sums, keys);
     };
@@ -590,7 +633,7 @@ extern "C" int ulm_token_logprobs_bwd(const void *logits, int dtype, const long 
     ULM_REQUIRE(logits && tokens && stats && dlogits && (!dentropy || entropy) && (!dtop || (top_tokens && top)),
                 "ulm_token_logprobs_bwd: null pointer");
     ULM_REQUIRE(dlogits != logits, "ulm_token_logprobs_bwd: dlogits must not alias logits");
-    const int tile = lp::kThreads * lp::kUnroll * (dtype == ULM_F32 ? 4 : 8), tiles = (V + tile - 1) / tile;
+    const int tile = lp::kThreads * (dtype == ULM_F32 ? 4 : 8), tiles = (V + tile - 1) / tile;
     const lp::Rows a{static_cast<const char *>(logits), tokens, inner, outer_stride, row_stride, ignore_index, rows, V, top, 1, V};
     const lp::Grads g{stats, entropy, dlogprob, dentropy, dtop, top_tokens, static_cast<char *>(dlogits)};
     hipStream_t s = static_cast<hipStream_t>(stream);

@@ -841,7 +841,7 @@ def token_logprobs_fwd(logits: Tensor, tokens: Tensor, top: int,
         with torch.cuda.device(logits.device):
             x, inner, outer_stride, row_stride = _rows(logits)
             tok = _int_tokens(tokens)
-            ws_bytes = nat.lib().ulm_token_logprobs_workspace_bytes(rows, V, top)
+            ws_bytes = nat.lib().ulm_token_logprobs_workspace_bytes(rows, V, top, nat.dtype_code(logits.dtype))
             ws = torch.empty(max(ws_bytes, 1), device=logits.device, dtype=torch.uint8)
             call("ulm_token_logprobs", ptr(x), nat.dtype_code(logits.dtype), ptr(tok), rows, inner, outer_stride,
                  row_stride, V, top, ignore_index, ptr(logprob), ptr(entropy), ptr(top_logprobs), ptr(top_tokens),

@@ -71,7 +71,7 @@ SIGNATURES = {
     "ulm_decode_step_workspace_bytes": (SZ, [I, I, I, I]),
     "ulm_decode_step": (I, [P, I, P, P, P, SZ, I, I, I, I, P]),
     "ulm_token_logprobs_max_top": (I, []),
-    "ulm_token_logprobs_workspace_bytes": (SZ, [L, I, I]),
+    "ulm_token_logprobs_workspace_bytes": (SZ, [L, I, I, I]),
     "ulm_token_logprobs": (I, [P, I, P, L, L, L, L, I, I, L, P, P, P, P, P, P, SZ, P]),
     "ulm_token_logprobs_bwd": (I, [P, I, P, L, L, L, L, I, I, L, P, P, P, P, P, P, P, P]),
     "ulm_embed_fwd": (I, [P, I, P, L, I, I, F, P, P]),
