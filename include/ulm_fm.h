@@ -423,7 +423,8 @@ int ulm_token_logprobs_bwd(const void *logits, int dtype, const long long *token
 /* Embedding lookup (nn.Embedding, model.py:117, 150) and its weight's gradient:
  * out[n] = scale W[tokens[n]], W (V,D) and out (N,D) dense in dtype; a token
  * outside [0, V) gives a row of NaN. dweight[v] = scale times the sum of dout[n]
- * over n with tokens[n] = v, in the order of n (fp32, rounded once), 0 for the
+ * over n with tokens[n] = v (fp32, rounded once; in the order of n, in chunks whose
+ * sums are added in order), 0 for the
  * tokens that do not occur; tokens outside [0, V) add to no row. Equal inputs
  * give equal bits. N at most 2^30. Workspace of ulm_embed_bwd_workspace_bytes() bytes. */
 int ulm_embed_fwd(const void *weight, int dtype, const long long *tokens, long long N, int V, int D, float scale,

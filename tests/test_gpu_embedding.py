@@ -97,7 +97,8 @@ def test_every_token_once_in_any_order():
 
 
 def test_sums_go_in_the_order_of_the_positions():
-    """Terms of 2^24 and 1: their fp32 sum depends on the order, which is the positions'."""
+    """Terms of 2^24 and 1: their fp32 sum depends on the order, which is the positions', 16 sorted
+    rows at a time in a short sequence, and then those sums'."""
     say("embedding order of the sums")
     weight, tokens, dout = make(24, 3, 4, "fp32", 9)
     tokens.copy_(torch.tensor([2, 0] * 12))
@@ -105,10 +106,10 @@ def test_sums_go_in_the_order_of_the_positions():
     dout[4], dout[20] = 2.0 ** 24, -2.0 ** 24
     w = weight.requires_grad_(True)
     g, = torch.autograd.grad(kernel.embedding(w, tokens), w, dout)
-    acc = torch.zeros(4)
-    for n in range(0, 24, 2):
-        acc = acc + dout[n].cpu()
-    assert torch.equal(g[2].cpu(), acc) and (g[0] == 12).all() and (g[1] == 0).all()
+    parts = [torch.zeros(4), torch.zeros(4)]   # token 2's rows are the sorted ones from the 12th on
+    for k, n in enumerate(range(0, 24, 2)):
+        parts[(12 + k) // 16] += dout[n].cpu()
+    assert torch.equal(g[2].cpu(), parts[0] + parts[1]) and (g[0] == 12).all() and (g[1] == 0).all()
 
 
 @pytest.mark.parametrize("N", [50, 5000])

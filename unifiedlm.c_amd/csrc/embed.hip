@@ -3,7 +3,7 @@
 //
 //     out[n] = scale W[t_n]      dW[v] = scale sum over n with t_n = v of dout[n]
 //
-// The gradient's rows are summed in the order of n: the tokens are sorted with their
+// The gradient's rows are summed in an order that the tokens fix: the tokens are sorted with their
 // positions by a stable radix sort, the rows of dout are summed along the sorted order in
 // chunks of equal length, one wave each, and sums that go over a chunk's end are
 // joined afterwards. No atomics on numbers: equal inputs give equal bits.
@@ -50,39 +50,86 @@ template <int DT> __device__ __forceinline__ u32x4_any pack(const float (&x)[Ele
     return w;
 }
 
-// elements [i, i + vec) of a row of D, zeros past its end
+// Vector p of a row of D elements: the row's last vector ends with it and overlaps the one before,
+// whose elements it computes as well, to the same bits. Rows shorter than a vector are one
+// vector, read and written by elements.
+template <int E> __device__ __forceinline__ int column(int p, int D) { return D < E ? 0 : min(p * E, D - E); }
+
 template <int DT> __device__ __forceinline__ void load_vec(const char *row, int i, int D, float (&x)[Elem<DT>::vec]) {
-    constexpr int V = Elem<DT>::vec;
-    if (i + V <= D) {
+    constexpr int E = Elem<DT>::vec;
+    if (D >= E) {
         unpack<DT>(*reinterpret_cast<const u32x4_any *>(row + static_cast<size_t>(i) * Elem<DT>::bytes), x);
     } else {
 #pragma unroll
-        for (int k = 0; k < V; ++k) x[k] = i + k < D ? load_as_f32(row, i + k, DT) : 0.f;
+        for (int k = 0; k < E; ++k) x[k] = k < D ? load_as_f32(row, k, DT) : 0.f;
     }
 }
 
-template <int DT> __device__ __forceinline__ void store_vec(char *row, int i, int D, const float (&x)[Elem<DT>::vec]) {
-    constexpr int V = Elem<DT>::vec;
-    if (i + V <= D) {
-        *reinterpret_cast<u32x4_any *>(row + static_cast<size_t>(i) * Elem<DT>::bytes) = pack<DT>(x);
+// the vector as it lies in memory, of a stream that the caches need not keep
+template <int DT> __device__ __forceinline__ u32x4_any load_raw(const char *row, int i, int D) {
+    constexpr int E = Elem<DT>::vec;
+    if (D >= E) return __builtin_nontemporal_load(reinterpret_cast<const u32x4_any *>(row + static_cast<size_t>(i) * Elem<DT>::bytes));
+    float x[E];
+    load_vec<DT>(row, i, D, x);
+    return pack<DT>(x);
+}
+
+template <int DT, bool STREAM = false>
+__device__ __forceinline__ void store_vec(char *row, int i, int D, const float (&x)[Elem<DT>::vec]) {
+    constexpr int E = Elem<DT>::vec;
+    if (D >= E) {
+        u32x4_any *to = reinterpret_cast<u32x4_any *>(row + static_cast<size_t>(i) * Elem<DT>::bytes);
+        if constexpr (STREAM) __builtin_nontemporal_store(pack<DT>(x), to);
+        else *to = pack<DT>(x);
     } else {
 #pragma unroll
-        for (int k = 0; k < V; ++k)
-            if (i + k < D) store_from_f32(row, i + k, DT, x[k]);
+        for (int k = 0; k < E; ++k)
+            if (k < D) store_from_f32(row, k, DT, x[k]);
     }
 }
 
-// ---- lookup: each thread one 16-byte piece of a row, pieces in order over the grid
+// the same of fp32 sums
+template <int E> __device__ __forceinline__ void load_sums(const float *row, int i, int D, float (&x)[E]) {
+    if (D >= E) {
+#pragma unroll
+        for (int k = 0; k < E; k += 4) {
+            const u32x4_any w = *reinterpret_cast<const u32x4_any *>(row + i + k);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) x[k + j] = __uint_as_float(w[j]);
+        }
+    } else {
+#pragma unroll
+        for (int k = 0; k < E; ++k) x[k] = k < D ? row[k] : 0.f;
+    }
+}
+template <int E> __device__ __forceinline__ void store_sums(float *row, int i, int D, const float (&x)[E]) {
+    if (D >= E) {
+#pragma unroll
+        for (int k = 0; k < E; k += 4) {
+            u32x4_any w;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) w[j] = __float_as_uint(x[k + j]);
+            *reinterpret_cast<u32x4_any *>(row + i + k) = w;
+        }
+    } else {
+#pragma unroll
+        for (int k = 0; k < E; ++k)
+            if (k < D) row[k] = x[k];
+    }
+}
+
+// ---- lookup: each thread one vector of a row, vectors in order over the grid
 
 template <int DT>
 __global__ __launch_bounds__(kThreads) void fwd_kernel(const char *__restrict__ weight, const long long *__restrict__ tokens,
-                                                       char *__restrict__ out, long long N, int V, int D, int pieces,
+                                                       char *__restrict__ out, long long N, int V, int D, uint32_t pieces,
                                                        float scale) {
     constexpr int E = Elem<DT>::vec, B = Elem<DT>::bytes;
     const long long total = N * pieces, step = static_cast<long long>(gridDim.x) * kThreads;
     for (long long p = static_cast<long long>(blockIdx.x) * kThreads + threadIdx.x; p < total; p += step) {
-        const long long n = p / pieces;
-        const int i = static_cast<int>(p % pieces) * E;
+        // 32-bit division where it will do
+        const long long n = total <= UINT32_MAX ? static_cast<uint32_t>(p) / pieces : p / pieces;
+        const int i = column<E>(static_cast<int>(p - n * pieces), D);
         const long long t = tokens[n];
         float x[E];
         if (t >= 0 && t < V) {
@@ -101,7 +148,8 @@ __global__ __launch_bounds__(kThreads) void fwd_kernel(const char *__restrict__ 
 
 constexpr int kBits = 10, kBins = 1 << kBits;
 constexpr int kSortThreads = 1024, kSortWaves = kSortThreads / kWave;
-constexpr int kTile = 4096;   // entries per workgroup of a pass
+constexpr int kTile = 4096;   // entries per workgroup of a long sequence's pass
+constexpr int kShort = 32768;   // tokens up to which a pass is one launch
 
 struct Entry {
     uint32_t token, pos;
@@ -120,17 +168,7 @@ struct Source {
     }
 };
 
-// counts[bin][tile]: the entries of each tile by their digit
-__global__ __launch_bounds__(kSortThreads) void count_kernel(Source src, int N, int shift, uint32_t *counts, int tiles) {
-    __shared__ uint32_t hist[kBins];
-    for (int b = threadIdx.x; b < kBins; b += kSortThreads) hist[b] = 0;
-    __syncthreads();
-    const int tile = blockIdx.x, end = min(N, (tile + 1) * kTile);
-    for (int i = tile * kTile + threadIdx.x; i < end; i += kSortThreads)
-        atomicAdd(&hist[(src.at(i).token >> shift) & (kBins - 1)], 1u);
-    __syncthreads();
-    for (int b = threadIdx.x; b < kBins; b += kSortThreads) counts[static_cast<size_t>(b) * tiles + tile] = hist[b];
-}
+__device__ __forceinline__ uint32_t digit_of(uint32_t token, int shift) { return (token >> shift) & (kBins - 1); }
 
 __device__ __forceinline__ uint32_t wave_scan(uint32_t v, int lane) {   // inclusive
 #pragma unroll
@@ -139,6 +177,17 @@ __device__ __forceinline__ uint32_t wave_scan(uint32_t v, int lane) {   // inclu
         if (lane >= off) v += o;
     }
     return v;
+}
+
+// counts[bin][tile]: the entries of each tile by their digit
+__global__ __launch_bounds__(kSortThreads) void count_kernel(Source src, int N, int shift, uint32_t *counts, int tiles) {
+    __shared__ uint32_t hist[kBins];
+    for (int b = threadIdx.x; b < kBins; b += kSortThreads) hist[b] = 0;
+    __syncthreads();
+    const int tile = blockIdx.x, end = min(N, (tile + 1) * kTile);
+    for (int i = tile * kTile + threadIdx.x; i < end; i += kSortThreads) atomicAdd(&hist[digit_of(src.at(i).token, shift)], 1u);
+    __syncthreads();
+    for (int b = threadIdx.x; b < kBins; b += kSortThreads) counts[static_cast<size_t>(b) * tiles + tile] = hist[b];
 }
 
 // Each bin's counts turned into the entries of that bin in earlier tiles, in place; totals[bin].
@@ -155,42 +204,75 @@ __global__ __launch_bounds__(kWave) void scan_kernel(uint32_t *counts, int tiles
     if (lane == 0) totals[blockIdx.x] = before;
 }
 
-// Every entry of a tile to its place: the smaller digits' total, the same digit's entries in
-// earlier tiles, in earlier waves of this tile, and among the lanes before.
+// Every entry of a tile of PER x kSortThreads to its place: the smaller digits' total, the same
+// digit's entries in earlier tiles, in earlier waves of this tile, and among the lanes before.
+// COUNT: the first two are counted here, by every workgroup, over the whole sequence, which for
+// a short one takes less time than two more launches (counts and totals are not used then).
+template <int PER, bool COUNT>
 __global__ __launch_bounds__(kSortThreads) void place_kernel(Source src, int N, int shift, const uint32_t *counts, int tiles,
                                                              const uint32_t *totals, Entry *out) {
     static_assert(kBins == kSortThreads, "one bin per thread");
-    constexpr int kPer = kTile / kSortThreads;   // 64-entry rows of a wave
-    __shared__ uint32_t base[kBins];
+    __shared__ uint32_t base[kBins], all[COUNT ? kBins : 1];
     __shared__ uint16_t seen[kSortWaves][kBins];   // a wave's entries of each digit, then those of the waves before it
     __shared__ uint32_t sums[kSortWaves];
-    const int tid = threadIdx.x, lane = tid % kWave, wave = tid / kWave, tile = blockIdx.x;
+    const int tid = threadIdx.x, lane = tid % kWave, wave = tid / kWave, tile = blockIdx.x, start = tile * PER * kSortThreads;
 
-    const uint32_t total = totals[tid], inc = wave_scan(total, lane);
-    if (lane == kWave - 1) sums[wave] = inc;
-    for (int w = 0; w < kSortWaves; ++w) seen[w][tid] = 0;
-    __syncthreads();
-    uint32_t below = inc - total;
-    for (int w = 0; w < wave; ++w) below += sums[w];
-    base[tid] = below + counts[static_cast<size_t>(tid) * tiles + tile];
-
-    Entry e[kPer];
-    uint32_t rank[kPer];
+    Entry e[PER];
 #pragma unroll
-    for (int k = 0; k < kPer; ++k) {
-        const int i = tile * kTile + (wave * kPer + k) * kWave + lane;
+    for (int k = 0; k < PER; ++k) {
+        const int i = start + (wave * PER + k) * kWave + lane;
+        e[k] = i < N ? src.at(i) : Entry{0, 0};
+    }
+    uint32_t *clear = reinterpret_cast<uint32_t *>(seen);
+    for (int i = tid; i < kSortWaves * kBins / 2; i += kSortThreads) clear[i] = 0;
+    static_assert(!COUNT || PER == 1, "tiles of one entry a thread");
+    if constexpr (COUNT) {
+        base[tid] = all[tid] = 0;
+        __syncthreads();
+        // Lanes that follow one of the same digit leave it to that one to count them: an earlier pass brings
+        // a frequent token's entries together, and a wave's additions to one counter go one by one.
+        constexpr int kRead = 16;
+        for (int i = 0; i < N; i += kRead * kSortThreads) {
+            uint32_t digit[kRead];
+#pragma unroll
+            for (int k = 0; k < kRead; ++k) digit[k] = digit_of(src.at(min(i + k * kSortThreads + tid, N - 1)).token, shift);
+#pragma unroll
+            for (int k = 0; k < kRead; ++k) {
+                const int at = i + k * kSortThreads;   // of the whole workgroup: a tile of one entry a thread
+                if (at >= N) break;
+                const uint32_t left = __shfl_up(digit[k], 1, kWave);
+                const uint64_t live = __ballot(at + tid < N), first = __ballot(lane == 0 || left != digit[k]) & live;
+                const uint64_t ends = (first | ~live) & ~((2ull << lane) - 1);   // the lanes above that end the run
+                if (first >> lane & 1)
+                    atomicAdd(&(at < start ? base : all)[digit[k]],
+                              static_cast<uint32_t>((ends ? __ffsll(static_cast<unsigned long long>(ends)) - 1 : kWave) - lane));
+            }
+        }
+    }
+    __syncthreads();
+    const uint32_t total = COUNT ? all[tid] + base[tid] : totals[tid], inc = wave_scan(total, lane);
+    if (lane == kWave - 1) sums[wave] = inc;
+    __syncthreads();
+    uint32_t below = lane < wave ? sums[lane] : 0;   // the waves' totals before this one's
+#pragma unroll
+    for (int off = kSortWaves / 2; off > 0; off >>= 1) below += __shfl_xor(below, off, kWave);
+    below = __builtin_amdgcn_readfirstlane(below) + inc - total;
+    if constexpr (COUNT) base[tid] += below;
+    else base[tid] = below + counts[static_cast<size_t>(tid) * tiles + tile];
+
+    uint32_t rank[PER];
+#pragma unroll
+    for (int k = 0; k < PER; ++k) {
+        const int i = start + (wave * PER + k) * kWave + lane;
         const bool live = i < N;
-        e[k] = live ? src.at(i) : Entry{0, 0};
-        const uint32_t digit = (e[k].token >> shift) & (kBins - 1);
+        const uint32_t digit = digit_of(e[k].token, shift);
         uint64_t same = __ballot(live);   // the lanes with this digit
-        if (!live) same = ~same;
 #pragma unroll
         for (int b = 0; b < kBits; ++b) {
             const uint64_t m = __ballot(digit >> b & 1);
             same &= (digit >> b & 1) ? m : ~m;
         }
-        const uint32_t ahead = __popcll(same & ((1ull << lane) - 1));
-        rank[k] = seen[wave][digit] + ahead;
+        rank[k] = seen[wave][digit] + __popcll(same & ((1ull << lane) - 1));
         // the wave's own counters: every lane has read them before the last lane of each digit writes
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         __builtin_amdgcn_wave_barrier();
@@ -199,25 +281,28 @@ __global__ __launch_bounds__(kSortThreads) void place_kernel(Source src, int N, 
         __builtin_amdgcn_wave_barrier();
     }
     __syncthreads();
+    uint16_t c[kSortWaves];
+#pragma unroll
+    for (int w = 0; w < kSortWaves; ++w) c[w] = seen[w][tid];
     uint32_t before = 0;
+#pragma unroll
     for (int w = 0; w < kSortWaves; ++w) {
-        const uint32_t c = seen[w][tid];
         seen[w][tid] = static_cast<uint16_t>(before);
-        before += c;
+        before += c[w];
     }
     __syncthreads();
 #pragma unroll
-    for (int k = 0; k < kPer; ++k) {
-        const int i = tile * kTile + (wave * kPer + k) * kWave + lane;
+    for (int k = 0; k < PER; ++k) {
+        const int i = start + (wave * PER + k) * kWave + lane;
         if (i >= N) continue;
-        const uint32_t digit = (e[k].token >> shift) & (kBins - 1);
+        const uint32_t digit = digit_of(e[k].token, shift);
         out[base[digit] + seen[wave][digit] + rank[k]] = e[k];
     }
 }
 
 // ---- the sums along the sorted order
 
-constexpr int kAhead = 8;   // rows of dout in flight per wave
+constexpr int kAhead = 8;   // rows of dout, or partial sums, in flight per wave
 
 // The first of the sorted entries lo .. N - 1 whose token is no less than t (N: none); the wave searches together, 65 ways a step.
 __device__ __forceinline__ int lower_bound(const Entry *e, int lo, int N, uint32_t t, int lane) {
@@ -235,7 +320,7 @@ __device__ __forceinline__ int lower_bound(const Entry *e, int lo, int N, uint32
 
 struct Sort {
     const Entry *entries;
-    int N, V, D, chunk, chunks;   // chunk entries a wave
+    int N, V, D, chunk, chunks, pieces;   // chunk entries a wave, pieces vectors a row
 };
 
 // One wave per (chunk, strip of 64 vectors of columns). Runs of one token inside the chunk are
@@ -245,7 +330,9 @@ template <int DT>
 __device__ __forceinline__ void sum_chunk(const Sort &s, const char *dout, char *dw, float *partial, float scale, int chunk,
                                           int strip, int lane) {
     constexpr int E = Elem<DT>::vec, B = Elem<DT>::bytes;
-    const int i0 = chunk * s.chunk, i1 = min(s.N, i0 + s.chunk), col = (strip * kWave + lane) * E;
+    const int i0 = chunk * s.chunk, i1 = min(s.N, i0 + s.chunk), piece = strip * kWave + lane;
+    const bool live = piece < s.pieces;
+    const int col = column<E>(live ? piece : s.pieces - 1, s.D);   // the others' loads: in the row, and dropped
     uint32_t token = s.entries[i0].token;
     const uint32_t last = s.entries[i1 - 1].token;
     bool open = i0 > 0 && s.entries[i0 - 1].token == token;      // the run began before
@@ -254,30 +341,36 @@ __device__ __forceinline__ void sum_chunk(const Sort &s, const char *dout, char 
 #pragma unroll
     for (int k = 0; k < E; ++k) acc[k] = 0.f;
     auto put_partial = [&](int slot) {
-#pragma unroll
-        for (int k = 0; k < E; ++k)
-            if (col + k < s.D) partial[(2 * static_cast<size_t>(chunk) + slot) * s.D + col + k] = acc[k];
+        if (live) store_sums(partial + (2 * static_cast<size_t>(chunk) + slot) * s.D, col, s.D, acc);
     };
     auto put_row = [&]() {
-        if (token >= static_cast<uint32_t>(s.V) || col >= s.D) return;
+        if (token >= static_cast<uint32_t>(s.V) || !live) return;
         float x[E];
 #pragma unroll
         for (int k = 0; k < E; ++k) x[k] = acc[k] * scale;
-        store_vec<DT>(dw + static_cast<size_t>(token) * s.D * B, col, s.D, x);
+        store_vec<DT, true>(dw + static_cast<size_t>(token) * s.D * B, col, s.D, x);
     };
-    for (int i = i0; i < i1; i += kAhead) {
-        float x[kAhead][E];
-        uint32_t tok[kAhead];
+    constexpr int A = kAhead;
+    u32x4_any w[A];
+    uint32_t tok[A], next_tok[A];
+    Entry mine{};   // 64 entries at once, lane by lane
+    auto load = [&](int i, u32x4_any (&to)[A], uint32_t (&t)[A]) {
+        if ((i - i0) % kWave == 0) mine = s.entries[min(i + lane, i1 - 1)];
 #pragma unroll
-        for (int j = 0; j < kAhead; ++j) {
-            const Entry e = s.entries[min(i + j, i1 - 1)];
-            tok[j] = e.token;
-            if (col < s.D) load_vec<DT>(dout + static_cast<size_t>(e.pos) * s.D * B, col, s.D, x[j]);
+        for (int j = 0; j < A; ++j) {
+            const int from = (i - i0) % kWave + j;
+            t[j] = __builtin_amdgcn_readlane(mine.token, from);
+            to[j] = load_raw<DT>(dout + static_cast<size_t>(__builtin_amdgcn_readlane(mine.pos, from)) * s.D * B, col, s.D);
         }
+    };
+    load(i0, w, tok);
+    for (int i = i0; i < i1; i += A) {
+        u32x4_any next[A];
+        if (i + A < i1) load(i + A, next, next_tok);   // on their way while these are summed
 #pragma unroll
-        for (int j = 0; j < kAhead; ++j) {
-            if (i + j >= i1) break;
-            if (tok[j] != token) {
+        for (int j = 0; j < A; ++j) {
+            const bool in = i + j < i1;
+            if (in && tok[j] != token) {
                 if (open) put_partial(0);
                 else put_row();
                 open = false;
@@ -285,8 +378,15 @@ __device__ __forceinline__ void sum_chunk(const Sort &s, const char *dout, char 
 #pragma unroll
                 for (int k = 0; k < E; ++k) acc[k] = 0.f;
             }
+            float x[E];
+            unpack<DT>(w[j], x);
 #pragma unroll
-            for (int k = 0; k < E; ++k) acc[k] += x[j][k];
+            for (int k = 0; k < E; ++k) acc[k] += in ? x[k] : 0.f;
+        }
+#pragma unroll
+        for (int j = 0; j < A; ++j) {
+            w[j] = next[j];
+            tok[j] = next_tok[j];
         }
     }
     if (open) put_partial(0);
@@ -294,7 +394,7 @@ __device__ __forceinline__ void sum_chunk(const Sort &s, const char *dout, char 
     else put_row();
 }
 
-constexpr int kZeroRows = 32;   // rows of dW a wave looks after: the absent ones are zeroed
+constexpr int kZeroRows = 8;   // rows of dW a wave looks after: the absent ones are zeroed
 
 template <int DT>
 __global__ __launch_bounds__(kThreads) void sum_kernel(Sort s, const char *dout, char *dw, float *partial, float scale,
@@ -327,55 +427,96 @@ __global__ __launch_bounds__(kThreads) void sum_kernel(Sort s, const char *dout,
     for (int k = 0; k < E; ++k) zero[k] = 0.f;
     for (int r = 0; r < rows; ++r) {
         if (present >> r & 1) continue;
-        for (int c = lane * E; c < s.D; c += kWave * E) store_vec<DT>(dw + static_cast<size_t>(v0 + r) * s.D * B, c, s.D, zero);
+        for (int p = lane; p < s.pieces; p += kWave)
+            store_vec<DT, true>(dw + static_cast<size_t>(v0 + r) * s.D * B, column<E>(p, s.D), s.D, zero);
     }
 }
 
-// Runs that go over chunks: the workgroup of the chunk in which one begins adds up its parts, each wave a
-// contiguous share of them and the waves' sums in order.
-template <int DT>
-__global__ __launch_bounds__(kThreads) void join_kernel(Sort s, char *dw, const float *partial, float scale, int strips) {
-    constexpr int E = Elem<DT>::vec, B = Elem<DT>::bytes, W = kThreads / kWave;
-    const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
-    const int chunk = blockIdx.x / strips, strip = blockIdx.x % strips, col = (strip * kWave + lane) * E;
-    const int i0 = chunk * s.chunk, i1 = i0 + s.chunk;
-    if (i1 >= s.N) return;
-    const uint32_t token = s.entries[i1 - 1].token;
-    if (token >= static_cast<uint32_t>(s.V) || s.entries[i1].token != token) return;   // no run goes on from here
-    if (s.entries[i0].token == token && i0 > 0 && s.entries[i0 - 1].token == token) return;   // it began earlier
-    const int end = lower_bound(s.entries, i1, s.N, token + 1, lane);
-    const int last = (end - 1) / s.chunk, parts = last - chunk + 1, each = (parts + W - 1) / W;
-    const int from = chunk + wave * each, to = min(last + 1, from + each);
-    float acc[E];
-#pragma unroll
-    for (int k = 0; k < E; ++k) acc[k] = 0.f;
+// Runs that go over chunks: a run's parts are added up where it begins. Each wave looks after one
+// (strip, chunk) and joins what its run left in up to kAlone chunks; a longer run's are joined by all
+// waves of the workgroup, each a contiguous share of them, and the waves' sums in order.
+// The workgroup's chunks follow each other, so that hardly more than one long run begins in them.
+constexpr int kJoinThreads = 512, kAlone = kAhead;
+
+template <int E>
+__device__ __forceinline__ void add_parts(const float *partial, int first, int from, int to, int col, int D, float (&acc)[E]) {
     for (int c = from; c < to; c += kAhead) {
         float x[kAhead][E];
 #pragma unroll
         for (int j = 0; j < kAhead; ++j) {
             const int cc = min(c + j, to - 1);
-            const float *p = partial + (2 * static_cast<size_t>(cc) + (cc == chunk)) * s.D;
-#pragma unroll
-            for (int k = 0; k < E; ++k) x[j][k] = col + k < s.D ? p[col + k] : 0.f;
+            load_sums(partial + (2 * static_cast<size_t>(cc) + (cc == first)) * D, col, D, x[j]);
         }
 #pragma unroll
         for (int j = 0; j < kAhead; ++j)
-            if (c + j < to)
 #pragma unroll
-                for (int k = 0; k < E; ++k) acc[k] += x[j][k];
+            for (int k = 0; k < E; ++k) acc[k] += c + j < to ? x[j][k] : 0.f;
     }
+}
+
+template <int DT>
+__global__ __launch_bounds__(kJoinThreads) void join_kernel(Sort s, char *dw, const float *partial, float scale, int strips) {
+    constexpr int E = Elem<DT>::vec, B = Elem<DT>::bytes, W = kJoinThreads / kWave;
+    const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
+    __shared__ int runs[W][2];   // each wave's run: its first and last chunk, where it is for all to join
+    __shared__ uint32_t tokens[W];
     __shared__ float part[W][kWave][E];
+
+    auto put = [&](uint32_t token, int col, float (&acc)[E]) {
 #pragma unroll
-    for (int k = 0; k < E; ++k) part[wave][lane][k] = acc[k];
+        for (int k = 0; k < E; ++k) acc[k] *= scale;
+        store_vec<DT, true>(dw + static_cast<size_t>(token) * s.D * B, col, s.D, acc);
+    };
+    // the run that begins in `chunk` and goes on behind it, if there is one: its token and last chunk
+    auto run_of = [&](int chunk, uint32_t &token, int &last) {
+        const int i0 = chunk * s.chunk, i1 = i0 + s.chunk;
+        if (i1 >= s.N) return false;
+        const uint32_t before = i0 > 0 ? s.entries[i0 - 1].token : ~0u, first = s.entries[i0].token;
+        const uint32_t after = s.entries[i1].token;
+        token = s.entries[i1 - 1].token;
+        if (token >= static_cast<uint32_t>(s.V) || after != token || (first == token && before == token)) return false;
+        for (last = chunk;;) {   // the last chunk that begins with it
+            const int c = last + 1 + lane;
+            const uint64_t same = __ballot(c < s.chunks && s.entries[min(c, s.chunks - 1) * s.chunk].token == token);
+            last += __popcll(same);
+            if (~same) return true;
+        }
+    };
+    const int id = blockIdx.x * W + wave, chunk = id % s.chunks;
+    uint32_t token = 0;
+    int last = 0;
+    const bool found = id < s.chunks * strips && run_of(chunk, token, last), alone = found && last - chunk < kAlone;
+    if (lane == 0) {
+        runs[wave][0] = found && !alone ? chunk : -1;
+        runs[wave][1] = last;
+        tokens[wave] = token;
+    }
+    if (alone) {
+        const int piece = id / s.chunks * kWave + lane, col = column<E>(min(piece, s.pieces - 1), s.D);
+        float acc[E] = {};
+        add_parts(partial, chunk, chunk, last + 1, col, s.D, acc);
+        if (piece < s.pieces) put(token, col, acc);
+    }
     __syncthreads();
-    if (wave || col >= s.D) return;
+    for (int w = 0; w < W; ++w) {
+        const int first = runs[w][0];
+        if (first < 0) continue;
+        const int parts = runs[w][1] - first + 1, each = (parts + W - 1) / W, from = first + wave * each;
+        const int piece = (blockIdx.x * W + w) / s.chunks * kWave + lane, col = column<E>(min(piece, s.pieces - 1), s.D);
+        float acc[E] = {};
+        add_parts(partial, first, from, min(first + parts, from + each), col, s.D, acc);
 #pragma unroll
-    for (int w = 1; w < W; ++w)
+        for (int k = 0; k < E; ++k) part[wave][lane][k] = acc[k];
+        __syncthreads();
+        if (wave == 0 && piece < s.pieces) {
 #pragma unroll
-        for (int k = 0; k < E; ++k) acc[k] += part[w][lane][k];
+            for (int v = 1; v < W; ++v)
 #pragma unroll
-    for (int k = 0; k < E; ++k) acc[k] *= scale;
-    store_vec<DT>(dw + static_cast<size_t>(token) * s.D * B, col, s.D, acc);
+                for (int k = 0; k < E; ++k) acc[k] += part[v][lane][k];
+            put(tokens[w], col, acc);
+        }
+        __syncthreads();
+    }
 }
 
 constexpr int kMaxV = 1 << 30;
@@ -386,7 +527,11 @@ inline int passes_of(int V) {   // the digits of 0 .. V
     while (bits < 31 && (static_cast<long long>(V) >> bits)) ++bits;
     return (bits + kBits - 1) / kBits;
 }
-inline int chunk_of(long long N) { return N <= 65536 ? 32 : 128; }
+inline int chunk_of(long long N) {   // about 1024 of them
+    int c = 16;
+    while (c < 512 && c * 1024LL < N) c *= 2;
+    return c;
+}
 
 struct Plan {
     Entry *a, *b;
@@ -453,11 +598,12 @@ extern "C" int ulm_embed_bwd(const void *dout, int dtype, const long long *token
     const size_t need = ulm_embed_bwd_workspace_bytes(N, V, D);
     ULM_REQUIRE(workspace_bytes >= need, "ulm_embed_bwd: workspace %zu < %zu", workspace_bytes, need);
     const int chunks = emb::plan(nullptr, N, D).chunks;
-    const int vec = dtype == ULM_F32 ? 4 : 8, strips = (D + vec * kWave - 1) / (vec * kWave), W = emb::kThreads / kWave;
+    const int vec = dtype == ULM_F32 ? 4 : 8, pieces = (D + vec - 1) / vec, strips = (pieces + kWave - 1) / kWave, W = emb::kThreads / kWave;
     const long long sum_blocks = (static_cast<long long>(chunks) * strips + W - 1) / W;
     const long long zero_blocks = (static_cast<long long>(V) + W * emb::kZeroRows - 1) / (W * emb::kZeroRows);
-    const long long join_blocks = static_cast<long long>(chunks) * strips;
-    ULM_REQUIRE(sum_blocks + zero_blocks < (1 << 24) && join_blocks < (1 << 24), "ulm_embed_bwd: N=%lld V=%d D=%d is too large", N, V, D);
+    constexpr int JW = emb::kJoinThreads / kWave;
+    const long long join_blocks = (static_cast<long long>(chunks) * strips + JW - 1) / JW;
+    ULM_REQUIRE(sum_blocks + zero_blocks < (1 << 24) && join_blocks < (1 << 23), "ulm_embed_bwd: N=%lld V=%d D=%d is too large", N, V, D);
     const emb::Plan p = emb::plan(workspace, N, D);
     hipStream_t st = static_cast<hipStream_t>(stream);
     const int n = static_cast<int>(N), passes = emb::passes_of(V);
@@ -465,18 +611,24 @@ extern "C" int ulm_embed_bwd(const void *dout, int dtype, const long long *token
     for (int k = 0; k < passes; ++k) {
         emb::Entry *to = k % 2 ? p.b : p.a;
         const int shift = k * emb::kBits;
-        emb::count_kernel<<<dim3(p.tiles), dim3(emb::kSortThreads), 0, st>>>(src, n, shift, p.counts, p.tiles);
-        emb::scan_kernel<<<dim3(emb::kBins), dim3(kWave), 0, st>>>(p.counts, p.tiles, p.totals);
-        emb::place_kernel<<<dim3(p.tiles), dim3(emb::kSortThreads), 0, st>>>(src, n, shift, p.counts, p.tiles, p.totals, to);
+        if (N <= emb::kShort) {
+            const dim3 grid((n + emb::kSortThreads - 1) / emb::kSortThreads);
+            emb::place_kernel<1, true><<<grid, dim3(emb::kSortThreads), 0, st>>>(src, n, shift, nullptr, 0, nullptr, to);
+        } else {
+            emb::count_kernel<<<dim3(p.tiles), dim3(emb::kSortThreads), 0, st>>>(src, n, shift, p.counts, p.tiles);
+            emb::scan_kernel<<<dim3(emb::kBins), dim3(kWave), 0, st>>>(p.counts, p.tiles, p.totals);
+            emb::place_kernel<emb::kTile / emb::kSortThreads, false><<<dim3(p.tiles), dim3(emb::kSortThreads), 0, st>>>(
+                src, n, shift, p.counts, p.tiles, p.totals, to);
+        }
         src = {nullptr, to, V};
     }
-    const emb::Sort s{src.entries, n, V, D, emb::chunk_of(N), p.chunks};
+    const emb::Sort s{src.entries, n, V, D, emb::chunk_of(N), p.chunks, pieces};
     emb::by_dtype(dtype, [&](auto dt) {
         constexpr int DT = decltype(dt)::value;
         emb::sum_kernel<DT><<<dim3(static_cast<unsigned>(sum_blocks + zero_blocks)), dim3(emb::kThreads), 0, st>>>(
             s, static_cast<const char *>(dout), static_cast<char *>(dweight), p.partial, scale, strips, static_cast<int>(sum_blocks));
         if (p.chunks > 1)
-            emb::join_kernel<DT><<<dim3(static_cast<unsigned>(join_blocks)), dim3(emb::kThreads), 0, st>>>(
+            emb::join_kernel<DT><<<dim3(static_cast<unsigned>(join_blocks)), dim3(emb::kJoinThreads), 0, st>>>(
                 s, static_cast<char *>(dweight), p.partial, scale, strips);
     });
     return check_launch("ulm_embed_bwd");

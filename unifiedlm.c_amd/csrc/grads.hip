@@ -17,13 +17,14 @@ namespace ulm {
 namespace gr {
 
 constexpr int kThreads = 256, kWaves = kThreads / kWave;
-constexpr int kVec = 8, kUnroll = 4;                        // elements a thread takes at once, and how many such
-constexpr int kChunk = kThreads * kVec * kUnroll;           // 8192 elements
+constexpr int kPer = 32;                                    // a thread's elements of a chunk
+constexpr int kChunk = kThreads * kPer;                     // 8192 elements
 constexpr int kBlocks = 1024;                               // workgroups of a norm launch at most
 constexpr int kTable = 112;                                 // tensors a launch takes: the arguments stay under 4 KB
 constexpr float kEps = 1e-6f;
 
 typedef uint32_t u32x4_any __attribute__((vector_size(16), aligned(2)));   // views start anywhere
+typedef uint32_t u32x2_any __attribute__((vector_size(8), aligned(2)));
 
 struct Table {
     const char *src[kTable];
@@ -45,68 +46,68 @@ __device__ __forceinline__ int tensor_of(const Table &t, uint32_t c) {
     return lo;
 }
 
-template <int DT> __device__ __forceinline__ void load8(const char *p, long long i, float (&x)[kVec]) {
+// V consecutive elements, 4 or 8: 16 bytes, or 8 of a 16-bit type where the other side has 32
+template <bool ONCE, class T> __device__ __forceinline__ T fetch(const char *p) {
+    if constexpr (ONCE) return __builtin_nontemporal_load(reinterpret_cast<const T *>(p));
+    else return *reinterpret_cast<const T *>(p);
+}
+template <int DT, int V, bool ONCE> __device__ __forceinline__ void load_vec(const char *p, long long i, float (&x)[V]) {
     if constexpr (DT == ULM_F32) {
-        const u32x4_any a = *reinterpret_cast<const u32x4_any *>(p + 4 * i), b = *reinterpret_cast<const u32x4_any *>(p + 4 * i + 16);
+        static_assert(V == 4, "16 bytes");
+        const u32x4_any w = fetch<ONCE, u32x4_any>(p + 4 * i);
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            x[k] = __uint_as_float(a[k]);
-            x[4 + k] = __uint_as_float(b[k]);
-        }
+        for (int k = 0; k < V; ++k) x[k] = __uint_as_float(w[k]);
     } else {
-        const u32x4_any a = *reinterpret_cast<const u32x4_any *>(p + 2 * i);
+        const auto w = fetch<ONCE, std::conditional_t<V == 8, u32x4_any, u32x2_any>>(p + 2 * i);
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
+        for (int k = 0; k < V / 2; ++k) {
             if constexpr (DT == ULM_BF16) {
-                x[2 * k] = __uint_as_float(a[k] << 16);
-                x[2 * k + 1] = __uint_as_float(a[k] & 0xffff0000u);
+                x[2 * k] = __uint_as_float(w[k] << 16);
+                x[2 * k + 1] = __uint_as_float(w[k] & 0xffff0000u);
             } else {
-                x[2 * k] = static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(a[k])));
-                x[2 * k + 1] = static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(a[k] >> 16)));
+                x[2 * k] = static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(w[k])));
+                x[2 * k + 1] = static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(w[k] >> 16)));
             }
         }
     }
 }
 
-template <int DT> __device__ __forceinline__ void store8(char *p, long long i, const float (&x)[kVec]) {
+template <int DT, int V> __device__ __forceinline__ void store_vec(char *p, long long i, const float (&x)[V]) {
     if constexpr (DT == ULM_F32) {
-        u32x4_any a, b;
+        u32x4_any w;
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            a[k] = __float_as_uint(x[k]);
-            b[k] = __float_as_uint(x[4 + k]);
-        }
-        *reinterpret_cast<u32x4_any *>(p + 4 * i) = a;
-        *reinterpret_cast<u32x4_any *>(p + 4 * i + 16) = b;
+        for (int k = 0; k < V; ++k) w[k] = __float_as_uint(x[k]);
+        __builtin_nontemporal_store(w, reinterpret_cast<u32x4_any *>(p + 4 * i));
     } else {
-        u32x4_any a;
+        using T = std::conditional_t<V == 8, u32x4_any, u32x2_any>;
+        T w;
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
+        for (int k = 0; k < V / 2; ++k) {
             if constexpr (DT == ULM_BF16)
-                a[k] = f32_to_bf16_bits(x[2 * k]) | (static_cast<uint32_t>(f32_to_bf16_bits(x[2 * k + 1])) << 16);
+                w[k] = f32_to_bf16_bits(x[2 * k]) | (static_cast<uint32_t>(f32_to_bf16_bits(x[2 * k + 1])) << 16);
             else
-                a[k] = __builtin_bit_cast(uint16_t, static_cast<_Float16>(x[2 * k])) |
+                w[k] = __builtin_bit_cast(uint16_t, static_cast<_Float16>(x[2 * k])) |
                        (static_cast<uint32_t>(__builtin_bit_cast(uint16_t, static_cast<_Float16>(x[2 * k + 1]))) << 16);
         }
-        *reinterpret_cast<u32x4_any *>(p + 2 * i) = a;
+        __builtin_nontemporal_store(w, reinterpret_cast<T *>(p + 2 * i));
     }
 }
 
-// a chunk's elements of a thread: kUnroll groups of 8, zeros past the tensor's end
-template <int DT>
-__device__ __forceinline__ void load_chunk(const char *p, long long base, long long numel, int tid, float (&x)[kUnroll][kVec]) {
+// a chunk's elements of a thread: vectors of V, zeros past the tensor's end
+template <int DT, int V, bool ONCE>
+__device__ __forceinline__ void load_chunk(const char *p, long long base, long long numel, int tid, float (&x)[kPer / V][V]) {
     if (base + kChunk <= numel) {
 #pragma unroll
-        for (int j = 0; j < kUnroll; ++j) load8<DT>(p, base + (j * kThreads + tid) * kVec, x[j]);
+        for (int j = 0; j < kPer / V; ++j) load_vec<DT, V, ONCE>(p, base + (j * kThreads + tid) * V, x[j]);
     } else {
 #pragma unroll
-        for (int j = 0; j < kUnroll; ++j) {
-            const long long i = base + (j * kThreads + tid) * kVec;
-            if (i + kVec <= numel) {
-                load8<DT>(p, i, x[j]);
+        for (int j = 0; j < kPer / V; ++j) {
+            const long long i = base + (j * kThreads + tid) * V;
+            if (i + V <= numel) {
+                load_vec<DT, V, ONCE>(p, i, x[j]);
             } else {
 #pragma unroll
-                for (int k = 0; k < kVec; ++k) x[j][k] = i + k < numel ? load_as_f32(p, i + k, DT) : 0.f;
+                for (int k = 0; k < V; ++k) x[j][k] = i + k < numel ? load_as_f32(p, i + k, DT) : 0.f;
             }
         }
     }
@@ -148,20 +149,27 @@ template <bool MAX> __device__ typename Acc<MAX>::T join(typename Acc<MAX>::T v)
     return v;
 }
 
+template <bool MAX, int DT>
+__device__ __forceinline__ typename Acc<MAX>::T take_chunk(typename Acc<MAX>::T acc, const char *p, long long base, long long numel) {
+    constexpr int V = DT == ULM_F32 ? 4 : 8;
+    float x[kPer / V][V];
+    load_chunk<DT, V, false>(p, base, numel, threadIdx.x, x);   // the caches keep what they can for the scaling
+#pragma unroll
+    for (int j = 0; j < kPer / V; ++j)
+#pragma unroll
+        for (int i = 0; i < V; ++i) acc = Acc<MAX>::take(acc, x[j][i]);
+    return acc;
+}
+
 template <bool MAX>
 __global__ __launch_bounds__(kThreads) void norm_kernel(Table t, typename Acc<MAX>::T *partial) {
     typename Acc<MAX>::T acc{};
     for (uint32_t c = blockIdx.x; c < t.first[t.n]; c += gridDim.x) {
         const int k = tensor_of(t, c);
         const long long base = static_cast<long long>(c - t.first[k]) * kChunk;
-        float x[kUnroll][kVec];
-        if (t.src_dt[k] == ULM_F32) load_chunk<ULM_F32>(t.src[k], base, t.numel[k], threadIdx.x, x);
-        else if (t.src_dt[k] == ULM_BF16) load_chunk<ULM_BF16>(t.src[k], base, t.numel[k], threadIdx.x, x);
-        else load_chunk<ULM_F16>(t.src[k], base, t.numel[k], threadIdx.x, x);
-#pragma unroll
-        for (int j = 0; j < kUnroll; ++j)
-#pragma unroll
-            for (int i = 0; i < kVec; ++i) acc = Acc<MAX>::take(acc, x[j][i]);
+        if (t.src_dt[k] == ULM_F32) acc = take_chunk<MAX, ULM_F32>(acc, t.src[k], base, t.numel[k]);
+        else if (t.src_dt[k] == ULM_BF16) acc = take_chunk<MAX, ULM_BF16>(acc, t.src[k], base, t.numel[k]);
+        else acc = take_chunk<MAX, ULM_F16>(acc, t.src[k], base, t.numel[k]);
     }
     acc = join<MAX>(acc);
     if (threadIdx.x == 0) partial[blockIdx.x] = acc;
@@ -182,19 +190,20 @@ __global__ __launch_bounds__(kThreads) void finish_kernel(const typename Acc<MAX
 
 template <int S, int D>
 __device__ __forceinline__ void scale_chunk(const char *src, char *dst, long long base, long long numel, float coef) {
+    constexpr int V = S == ULM_F32 || D == ULM_F32 ? 4 : 8;
     const int tid = threadIdx.x;
-    float x[kUnroll][kVec];
-    load_chunk<S>(src, base, numel, tid, x);
+    float x[kPer / V][V];
+    load_chunk<S, V, true>(src, base, numel, tid, x);
 #pragma unroll
-    for (int j = 0; j < kUnroll; ++j) {
-        const long long i = base + (j * kThreads + tid) * kVec;
+    for (int j = 0; j < kPer / V; ++j) {
+        const long long i = base + (j * kThreads + tid) * V;
 #pragma unroll
-        for (int k = 0; k < kVec; ++k) x[j][k] *= coef;
-        if (i + kVec <= numel) {
-            store8<D>(dst, i, x[j]);
+        for (int k = 0; k < V; ++k) x[j][k] *= coef;
+        if (i + V <= numel) {
+            store_vec<D, V>(dst, i, x[j]);
         } else {
 #pragma unroll
-            for (int k = 0; k < kVec; ++k)
+            for (int k = 0; k < V; ++k)
                 if (i + k < numel) store_from_f32(dst, i + k, D, x[j][k]);
         }
     }

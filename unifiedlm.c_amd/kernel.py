@@ -1005,7 +1005,8 @@ def embedding(weight, tokens, scale=1.0):
     """scale * weight[tokens]: weight (V, D) fp32, bf16 or fp16, tokens (...) integer, the result
     (..., D) in the weight's dtype, rounded once. A token outside [0, V) gives a row of NaN.
     The weight's gradient is dense, in its dtype: each row the fp32 sum of its tokens' gradients in
-    their order, so that equal inputs give equal bits; tokens outside [0, V) add nothing."""
+    an order that the tokens alone fix, so that equal inputs give equal bits; tokens outside [0, V) add
+    nothing."""
     if _plain_eager():
         out = nat.host().embedding(weight, tokens, scale)
         if out is not None:
