@@ -119,7 +119,7 @@ def test_the_entries_refuse_before_any_hip_call():
         x, nat.ULM_F32, X, 4, 4, 0, 10, 10, 0, -1, X, ent, X, X, dent, dtop, out, None)
     for a, msg in ((bw(out=X), b"alias"), (bw(out=None), b"null"), (bw(dtop=X), b"null"), (bw(dent=X, ent=None), b"null")):
         assert lib.ulm_token_logprobs_bwd(*a) == nat.ULM_ERR_INVALID and msg in lib.ulm_last_error()
-    assert lib.ulm_token_logprobs_max_top() == 64
+    assert lib.ulm_token_logprobs_max_top() == kernel.MAX_TOP == 64
     for a, msg in (((X, 9, X, 4, 10, 8, 1.0, X, None), b"bad dtype"), ((X, 0, X, 0, 10, 8, 1.0, X, None), b"bad sizes"),
                    ((X, 0, None, 4, 10, 8, 1.0, X, None), b"null"), ((X, 0, X, (1 << 30) + 1, 10, 8, 1.0, X, None), b"bad sizes")):
         assert lib.ulm_embed_fwd(*a) == nat.ULM_ERR_INVALID and msg in lib.ulm_last_error()

@@ -800,6 +800,7 @@ def decode_deferred(S, pv, pr, m, flush, q, g, x, ymu, cj=None):
 # model.py:160-161), with each row's entropy and its largest entries
 
 TokenLogprobs = namedtuple("TokenLogprobs", "logprob entropy top_logprobs top_tokens")
+MAX_TOP = 64   # ulm_token_logprobs_max_top()
 
 
 def _int_tokens(tokens):
@@ -934,7 +935,7 @@ def token_logprobs(logits, tokens, top=0, ignore_index=-1):
         raise ValueError(f"logits must be (..., V), got {tuple(logits.shape)}")
     if tokens.shape != logits.shape[:-1]:
         raise ValueError(f"tokens {tuple(tokens.shape)} must have the logits' leading shape, {tuple(logits.shape)}")
-    most = min(logits.shape[-1], nat.lib().ulm_token_logprobs_max_top())
+    most = min(logits.shape[-1], MAX_TOP)
     if not 0 <= top <= most:
         raise ValueError(f"top must be between 0 and {most}, got {top}")
     nat.dtype_code(logits.dtype)

@@ -18,6 +18,8 @@ weights). Every body here is this package's own:
 The reference's training-loop and sampling helpers keep their signatures
 (configure_optimizers, estimate_mfu, generate: train.py:172, 295, sample.py:61)
 with bodies of this package's own; generate samples on the decode kernels.
+`loss`, `score` and `clip_grad_norm_` run the ends of a training or scoring
+step on the package's kernels as well.
 """
 import inspect
 import math
@@ -28,9 +30,10 @@ import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
-from kernel import (CHUNK, LOG_W_MAX, LOG_W_MIN, block_eager, block_prefill, block_prefill_eager, decode_addr,
-                    decode_addr_deferred, decode_deferred, decode_pre, decode_state, decode_step, fm_prefill,
-                    matrix_copies, relu2_address, rms_norm, unified_block, unified_memory)
+from kernel import (CHUNK, LOG_W_MAX, LOG_W_MIN, TokenLogprobs, block_eager, block_prefill, block_prefill_eager,
+                    clip_grad_norm_, decode_addr, decode_addr_deferred, decode_deferred, decode_pre, decode_state,
+                    decode_step, embedding, fm_prefill, matrix_copies, relu2_address, rms_norm, token_logprobs,
+                    unified_block, unified_memory)
 
 # whether any hook is registered for every module (assumed where torch does not say)
 _any_global_hook = getattr(nn.modules.module, "_has_any_global_hook", lambda: True)
@@ -342,6 +345,51 @@ class UnifiedLM(nn.Module):
         logits = self.output(h)
         self.last_loss = F.cross_entropy(logits.flatten(0, 1), targets.flatten(), ignore_index=-1)
         return logits
+
+    def _hidden(self, tokens):
+        """What the classifier reads (B, T, dim), the embedding's rows gathered (and its gradient
+        summed in a fixed order) by kernel.embedding."""
+        h = self.dropout(embedding(self.tok_embeddings.weight, tokens))
+        for layer in self.layers:
+            h = layer(h)
+        return self.norm(h)
+
+    def loss(self, tokens: torch.Tensor, targets: torch.Tensor, entropy_weight: float = 0.0) -> torch.Tensor:
+        """The training loss of `forward` with targets (the mean cross-entropy over the targets that are
+        not -1, NaN where there are none) on kernel.embedding and kernel.token_logprobs: the
+        logits are read once for the loss and once for their gradient, in the dtype the classifier
+        gives them (bf16 under bf16 autocast), without the fp32 copies of a log-softmax. entropy_weight
+        takes that share of the same positions' mean entropy off it. last_loss is set as by `forward`."""
+        if targets.shape != tokens.shape:
+            raise ValueError(f"targets {tuple(targets.shape)} must have the tokens' shape {tuple(tokens.shape)}")
+        out = token_logprobs(self.output(self._hidden(tokens)), targets)
+        counted = targets != -1
+        loss = -out.logprob.sum() / counted.sum()
+        if entropy_weight:
+            loss = loss - entropy_weight * (out.entropy * counted).sum() / counted.sum()
+        self.last_loss = loss
+        return loss
+
+    @torch.no_grad()
+    def score(self, tokens: torch.Tensor, targets: Optional[torch.Tensor] = None, top: int = 0) -> TokenLogprobs:
+        """Log probabilities of given tokens (kernel.token_logprobs): of `targets` (B, T; -1 for those that do
+        not count) at the positions of tokens (B, T), or without targets of each token after the first
+        under the ones before it, (B, T - 1). With them every position's entropy and its `top` most
+        likely tokens."""
+        if targets is None:
+            tokens, targets = tokens[:, :-1], tokens[:, 1:]
+        elif targets.shape != tokens.shape:
+            raise ValueError(f"targets {tuple(targets.shape)} must have the tokens' shape {tuple(tokens.shape)}")
+        if tokens.numel() == 0:   # nothing to score
+            logits = self.output.weight.new_empty(*tokens.shape, self.params.vocab_size)
+        else:
+            logits = self.output(self._hidden(tokens))
+        return token_logprobs(logits, targets, top)
+
+    def clip_grad_norm_(self, max_norm: float, norm_type: float = 2.0, error_if_nonfinite: bool = False) -> torch.Tensor:
+        """kernel.clip_grad_norm_ of the model's parameters, as the training loop clips before its
+        optimizer's step; returns the norm the gradients had."""
+        return clip_grad_norm_(self.parameters(), max_norm, norm_type, error_if_nonfinite)
 
     def init_states(self, batch: int, device):
         return [layer.init_state(batch, device) for layer in self.layers]
