@@ -397,6 +397,7 @@ int ulm_decode_step(const ulm_decode_layer *layers, int n_layers, const float *x
  *   top_logprobs (rows, top) out: the `top` largest entries' log probabilities,
  *   top_tokens   (rows, top) out: and their indices; the lower index first on ties, a NaN
  *                            above all numbers. top at most ulm_token_logprobs_max_top() and V
+ *                            (V at most 2^30, 2^22 with top)
  *   stats        (rows, 2)   out: the row's maximum and ln sum_i e^(x_i - max), for the backward;
  *                            NULL: not wanted
  * A row of -inf only has logprob and top_logprobs -inf (0 if ignored), entropy 0, top_tokens
@@ -426,7 +427,7 @@ int ulm_token_logprobs_bwd(const void *logits, int dtype, const long long *token
  * over n with tokens[n] = v (fp32, rounded once; in the order of n, in chunks whose
  * sums are added in order), 0 for the
  * tokens that do not occur; tokens outside [0, V) add to no row. Equal inputs
- * give equal bits. N at most 2^30. Workspace of ulm_embed_bwd_workspace_bytes() bytes. */
+ * give equal bits. N at most 2^30, V 2^28, D 2^20. Workspace of ulm_embed_bwd_workspace_bytes() bytes. */
 int ulm_embed_fwd(const void *weight, int dtype, const long long *tokens, long long N, int V, int D, float scale,
                   void *out, void *stream);
 size_t ulm_embed_bwd_workspace_bytes(long long N, int V, int D);

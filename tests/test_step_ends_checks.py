@@ -33,6 +33,13 @@ def test_token_logprobs_refuses():
         kernel.token_logprobs(x[..., :0], t)
     with pytest.raises(TypeError, match="tensor"):
         kernel.token_logprobs(None, t)
+    with pytest.raises(TypeError):
+        kernel.token_logprobs(x, t, 1.5)
+    wide = torch.zeros(1).expand(1, (1 << 22) + 1)   # no memory behind it
+    with pytest.raises(ValueError, match="2\\^22"):
+        kernel.token_logprobs(wide, t[0, :1], 1)
+    with pytest.raises(ValueError, match="2\\^30"):
+        kernel.token_logprobs(torch.zeros(1).expand(1, (1 << 30) + 1), t[0, :1])
 
 
 def test_embedding_refuses():
@@ -47,6 +54,10 @@ def test_embedding_refuses():
         kernel.embedding(w, t.float())
     with pytest.raises(TypeError, match="scale"):
         kernel.embedding(w, t, torch.ones(()))
+    with pytest.raises(ValueError, match="2\\^28"):
+        kernel.embedding(torch.zeros(1).expand((1 << 28) + 1, 1), t)
+    with pytest.raises(ValueError, match="2\\^20"):
+        kernel.embedding(torch.zeros(1).expand(1, (1 << 20) + 1), t)
     for bad in (w[0], w[:0], w[:, :0], w[None]):
         with pytest.raises(ValueError, match=r"\(V, D\)"):
             kernel.embedding(bad, t)
@@ -113,7 +124,8 @@ def test_the_entries_refuse_before_any_hip_call():
         x, dt, X, rows, inner, 0, 10, V, top, -1, X, X, X, X, X, ws, n, None)
     for kw, msg in ((dict(rows=0), b"bad sizes"), (dict(V=0), b"bad sizes"), (dict(inner=0), b"bad sizes"), (dict(top=11), b"top"),
                     (dict(top=-1), b"top"), (dict(V=100, top=65), b"top"), (dict(dt=7), b"bad dtype"),
-                    (dict(x=None), b"null pointer"), (dict(V=1 << 20, n=0), b"workspace")):
+                    (dict(x=None), b"null pointer"), (dict(V=1 << 20, top=1, n=0), b"workspace"),
+                    (dict(V=(1 << 22) + 1, top=1), b"top=1 with")):
         assert lp(*args(**kw)) == nat.ULM_ERR_INVALID and msg in lib.ulm_last_error(), kw
     bw = lambda x=X, out=ctypes.c_void_p(512), dtop=None, dent=None, ent=X: (  # noqa: E731
         x, nat.ULM_F32, X, 4, 4, 0, 10, 10, 0, -1, X, ent, X, X, dent, dtop, out, None)

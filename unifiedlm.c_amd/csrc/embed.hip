@@ -519,7 +519,7 @@ __global__ __launch_bounds__(kJoinThreads) void join_kernel(Sort s, char *dw, co
     }
 }
 
-constexpr int kMaxV = 1 << 30;
+constexpr int kMaxV = 1 << 28, kMaxD = 1 << 20;
 constexpr long long kMaxN = 1LL << 30;
 
 inline int passes_of(int V) {   // the digits of 0 .. V
@@ -556,7 +556,7 @@ inline Plan plan(void *ws, long long N, int D) {
 
 int check(const char *fn, int dtype, long long N, int V, int D) {
     if (!valid_dtype(dtype)) return fail(ULM_ERR_INVALID, "%s: bad dtype %d", fn, dtype);
-    if (N < 1 || N > kMaxN || V < 1 || V > kMaxV || D < 1 || D > (1 << 24))
+    if (N < 1 || N > kMaxN || V < 1 || V > kMaxV || D < 1 || D > kMaxD)
         return fail(ULM_ERR_INVALID, "%s: bad sizes N=%lld V=%d D=%d", fn, N, V, D);
     return ULM_OK;
 }
@@ -587,7 +587,7 @@ extern "C" int ulm_embed_fwd(const void *weight, int dtype, const long long *tok
 }
 
 extern "C" size_t ulm_embed_bwd_workspace_bytes(long long N, int V, int D) {
-    if (N < 1 || N > emb::kMaxN || V < 1 || V > emb::kMaxV || D < 1 || D > (1 << 24)) return 0;
+    if (N < 1 || N > emb::kMaxN || V < 1 || V > emb::kMaxV || D < 1 || D > emb::kMaxD) return 0;
     return emb::plan(nullptr, N, D).bytes;
 }
 

@@ -662,7 +662,7 @@ py::object token_logprobs(const py::handle &logits_, const py::handle &tokens_, 
     if (!plain_thread() || !PyLong_CheckExact(top_.ptr()) || !PyLong_CheckExact(ignore_.ptr())) return py::none();
     const Tensor logits = plain(logits_), tokens = plain_ids(tokens_);
     if (!logits.defined() || !tokens.defined() || !has_code(logits) || logits.device() != tokens.device() || logits.dim() < 1 ||
-        logits.size(-1) == 0 || logits.size(-1) > INT32_MAX || tokens.sizes() != logits.sizes().slice(0, logits.dim() - 1))
+        logits.size(-1) == 0 || logits.size(-1) > (1 << 22) || tokens.sizes() != logits.sizes().slice(0, logits.dim() - 1))
         return py::none();
     const int64_t top = top_.cast<int64_t>(), ignore = ignore_.cast<int64_t>();
     if (top < 0 || top > std::min<int64_t>(logits.size(-1), ulm_token_logprobs_max_top())) return py::none();
@@ -728,7 +728,7 @@ py::object embedding(const py::handle &weight_, const py::handle &tokens_, const
     if (!plain_thread() || !(PyFloat_CheckExact(scale_.ptr()) || PyLong_CheckExact(scale_.ptr()))) return py::none();
     const Tensor weight = plain(weight_), tokens = plain_ids(tokens_);
     if (!weight.defined() || !tokens.defined() || !has_code(weight) || weight.device() != tokens.device() || weight.dim() != 2 ||
-        weight.numel() == 0 || weight.size(0) > (1 << 30) || tokens.numel() > (1 << 30) || weight.size(1) > (1 << 24))
+        weight.numel() == 0 || weight.size(0) > (1 << 28) || tokens.numel() > (1 << 30) || weight.size(1) > (1 << 20))
         return py::none();
     const double scale = scale_.cast<double>();
     return py::cast(unlocked([&] {

@@ -450,7 +450,8 @@ constexpr int kThreads = 256;   // of the kernels below
 // The parts of a row joined: one workgroup per row.
 template <int DT, bool TOP>
 __global__ __launch_bounds__(kThreads) void join_kernel(Rows a, Outs o, const Sums *part_sums, const uint64_t *part_keys) {
-    const long long r = blockIdx.x;
+    const long long r = block_id();
+    if (r >= a.rows) return;
     const int tid = threadIdx.x;
     __shared__ float ml[2];
     __shared__ uint64_t list[TOP ? kMaxParts * kMaxTop : 1];

@@ -19,6 +19,7 @@ lookup, the log probabilities of given tokens (the loss), and the gradients'
 norm and clipping.
 """
 import math
+import operator
 from collections import namedtuple
 from typing import Optional
 
@@ -935,9 +936,12 @@ def token_logprobs(logits, tokens, top=0, ignore_index=-1):
         raise ValueError(f"logits must be (..., V), got {tuple(logits.shape)}")
     if tokens.shape != logits.shape[:-1]:
         raise ValueError(f"tokens {tuple(tokens.shape)} must have the logits' leading shape, {tuple(logits.shape)}")
-    most = min(logits.shape[-1], MAX_TOP)
-    if not 0 <= top <= most:
-        raise ValueError(f"top must be between 0 and {most}, got {top}")
+    V = logits.shape[-1]
+    top, ignore_index = operator.index(top), operator.index(ignore_index)
+    if not 0 <= top <= min(V, MAX_TOP):
+        raise ValueError(f"top must be between 0 and {min(V, MAX_TOP)}, got {top}")
+    if V > 1 << 30 or (top and V > 1 << 22):
+        raise ValueError(f"at most 2^30 columns, 2^22 with alternatives, got {V}")
     nat.dtype_code(logits.dtype)
     nat.require_device(logits, tokens)
     return TokenLogprobs(*token_logprobs_fwd(logits, tokens, top, ignore_index)[:4])
@@ -1020,8 +1024,8 @@ def embedding(weight, tokens, scale=1.0):
     _check_tokens(tokens)
     if weight.dim() != 2 or weight.numel() == 0:
         raise ValueError(f"weight must be a non-empty (V, D), got {tuple(weight.shape)}")
-    if weight.shape[0] > 1 << 30 or tokens.numel() > 1 << 30:
-        raise ValueError(f"at most 2^30 tokens: weight {tuple(weight.shape)}, {tokens.numel()} tokens")
+    if weight.shape[0] > 1 << 28 or weight.shape[1] > 1 << 20 or tokens.numel() > 1 << 30:
+        raise ValueError(f"weight at most 2^28 x 2^20 and 2^30 tokens, got {tuple(weight.shape)} and {tokens.numel()}")
     nat.dtype_code(weight.dtype)
     nat.require_device(weight, tokens)
     return embed_fwd(weight, tokens, float(scale))
