@@ -76,11 +76,12 @@ def test_frequent_tokens(N, V, D, skew, dt):
     check(weight, tokens, math.sqrt(D), dout)
 
 
-@pytest.mark.parametrize("where", [0, 511, 512, 999])
-def test_one_token_throughout(where):
+@pytest.mark.parametrize("N,V,where", [(10000, 1000, 0), (10000, 1000, 511), (10000, 1000, 512), (10000, 1000, 999),
+                                       (10000, 5000, 4999), (32768, 32767, 32766), (32769, 32767, 7), (20000, 40000, 39999)])
+def test_one_token_throughout(N, V, where):
     """All rows one token, but for another at the first or last place: runs over every chunk."""
-    say(f"embedding one token throughout, V=1000, at {where}")
-    weight, tokens, dout = make(10000, 1000, 48, "fp32", 5)
+    say(f"embedding one token throughout, N={N} V={V}, at {where}")
+    weight, tokens, dout = make(N, V, 48, "fp32", 5)
     tokens.fill_(where)
     check(weight, tokens, 0.5, dout)
     tokens[0], tokens[-1] = 3, 998
@@ -112,11 +113,12 @@ def test_sums_go_in_the_order_of_the_positions():
     assert torch.equal(g[2].cpu(), parts[0] + parts[1]) and (g[0] == 12).all() and (g[1] == 0).all()
 
 
-@pytest.mark.parametrize("N", [50, 5000])
-def test_unknown_tokens(N):
-    say(f"embedding unknown tokens N={N}")
-    weight, tokens, dout = make(N, 1023, 33, "fp32", 11)
-    tokens[0], tokens[5], tokens[N - 1] = -1, 1023, 1 << 40
+@pytest.mark.parametrize("V", [1023, 1024, 5000, 32767, 32768])   # a digit, a digit and one, one launch's most, and one more
+@pytest.mark.parametrize("N", [50, 5000, 40000])
+def test_unknown_tokens(N, V):
+    say(f"embedding unknown tokens N={N} V={V}")
+    weight, tokens, dout = make(N, V, 33, "fp32", 11)
+    tokens[0], tokens[5], tokens[7], tokens[N - 1] = -1, V, V - 1, 1 << 40
     check(weight, tokens, 2.0, dout)
     tokens.fill_(-100)
     check(weight, tokens, 1.0, dout)

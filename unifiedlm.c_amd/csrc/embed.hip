@@ -68,7 +68,8 @@ template <int DT> __device__ __forceinline__ void load_vec(const char *row, int 
 // the vector as it lies in memory, of a stream that the caches need not keep
 template <int DT> __device__ __forceinline__ u32x4_any load_raw(const char *row, int i, int D) {
     constexpr int E = Elem<DT>::vec;
-    if (D >= E) return __builtin_nontemporal_load(reinterpret_cast<const u32x4_any *>(row + static_cast<size_t>(i) * Elem<DT>::bytes));
+    const char *p = row + static_cast<size_t>(i) * Elem<DT>::bytes;
+    if (D >= E) return __builtin_nontemporal_load(reinterpret_cast<const u32x4_any *>(p));
     float x[E];
     load_vec<DT>(row, i, D, x);
     return pack<DT>(x);
@@ -149,7 +150,7 @@ __global__ __launch_bounds__(kThreads) void fwd_kernel(const char *__restrict__ 
 constexpr int kBits = 10, kBins = 1 << kBits;
 constexpr int kSortThreads = 1024, kSortWaves = kSortThreads / kWave;
 constexpr int kTile = 4096;   // entries per workgroup of a long sequence's pass
-constexpr int kShort = 32768;   // tokens up to which a pass is one launch
+constexpr int kShort = 32768;   // tokens up to which a pass is one launch (at 65536 as long as three); half a counter holds them
 
 struct Entry {
     uint32_t token, pos;
@@ -179,13 +180,29 @@ __device__ __forceinline__ uint32_t wave_scan(uint32_t v, int lane) {   // inclu
     return v;
 }
 
+// How many lanes, this one first, hold `value` one after the other; 0 on a lane that follows another of its
+// run or is not live. Live lanes come first. What counts equal values adds a run at once: additions to
+// one counter go one by one, and a frequent token's entries come together (padding, or an earlier pass).
+__device__ __forceinline__ uint32_t run_length(uint32_t value, bool live, int lane) {
+    const uint32_t left = __shfl_up(value, 1, kWave);
+    const uint64_t in = __ballot(live), first = __ballot(lane == 0 || left != value) & in;
+    const uint64_t ends = (first | ~in) & ~((2ull << lane) - 1);   // the lanes above that end the run
+    const int end = ends ? __ffsll(static_cast<unsigned long long>(ends)) - 1 : kWave;
+    return first >> lane & 1 ? end - lane : 0;
+}
+
 // counts[bin][tile]: the entries of each tile by their digit
 __global__ __launch_bounds__(kSortThreads) void count_kernel(Source src, int N, int shift, uint32_t *counts, int tiles) {
     __shared__ uint32_t hist[kBins];
     for (int b = threadIdx.x; b < kBins; b += kSortThreads) hist[b] = 0;
     __syncthreads();
     const int tile = blockIdx.x, end = min(N, (tile + 1) * kTile);
-    for (int i = tile * kTile + threadIdx.x; i < end; i += kSortThreads) atomicAdd(&hist[digit_of(src.at(i).token, shift)], 1u);
+    for (int i = tile * kTile; i < end; i += kSortThreads) {
+        const int at = i + threadIdx.x;
+        const uint32_t digit = digit_of(src.at(min(at, end - 1)).token, shift);
+        const uint32_t run = run_length(digit, at < end, threadIdx.x % kWave);
+        if (run) atomicAdd(&hist[digit], run);
+    }
     __syncthreads();
     for (int b = threadIdx.x; b < kBins; b += kSortThreads) counts[static_cast<size_t>(b) * tiles + tile] = hist[b];
 }
@@ -229,8 +246,6 @@ __global__ __launch_bounds__(kSortThreads) void place_kernel(Source src, int N, 
     if constexpr (COUNT) {
         base[tid] = all[tid] = 0;
         __syncthreads();
-        // Lanes that follow one of the same digit leave it to that one to count them: an earlier pass brings
-        // a frequent token's entries together, and a wave's additions to one counter go one by one.
         constexpr int kRead = 16;
         for (int i = 0; i < N; i += kRead * kSortThreads) {
             uint32_t digit[kRead];
@@ -240,12 +255,8 @@ __global__ __launch_bounds__(kSortThreads) void place_kernel(Source src, int N, 
             for (int k = 0; k < kRead; ++k) {
                 const int at = i + k * kSortThreads;   // of the whole workgroup: a tile of one entry a thread
                 if (at >= N) break;
-                const uint32_t left = __shfl_up(digit[k], 1, kWave);
-                const uint64_t live = __ballot(at + tid < N), first = __ballot(lane == 0 || left != digit[k]) & live;
-                const uint64_t ends = (first | ~live) & ~((2ull << lane) - 1);   // the lanes above that end the run
-                if (first >> lane & 1)
-                    atomicAdd(&(at < start ? base : all)[digit[k]],
-                              static_cast<uint32_t>((ends ? __ffsll(static_cast<unsigned long long>(ends)) - 1 : kWave) - lane));
+                const uint32_t run = run_length(digit[k], at + tid < N, lane);
+                if (run) atomicAdd(&(at < start ? base : all)[digit[k]], run);
             }
         }
     }
@@ -300,11 +311,81 @@ __global__ __launch_bounds__(kSortThreads) void place_kernel(Source src, int N, 
     }
 }
 
+// The whole sort of a short sequence of tokens below kSmallV in one launch: every workgroup
+// counts all tokens, those of earlier tiles in the counter's upper half, turns the counts
+// into the places where its tile's entries begin, and its waves take theirs in turn. At 16384 tokens 12 us,
+// where the two digits' launches take 18 (the whole gradient 47 and 54, at 32768 47 and 58).
+constexpr int kSmallV = (1 << 15) - 1;   // tokens 0 .. kSmallV, the last one for those outside
+__global__ __launch_bounds__(kSortThreads) void place_small_kernel(Source src, int N, Entry *out) {
+    constexpr int kSmallBins = kSmallV + 1, kPer = kSmallBins / kSortThreads, kRead = 16;
+    __shared__ uint32_t bins[kSmallBins + kSortThreads];   // a word between threads' shares, off the same bank
+    __shared__ uint32_t sums[kSortWaves];
+    const int tid = threadIdx.x, lane = tid % kWave, wave = tid / kWave, start = blockIdx.x * kSortThreads;
+    auto bin = [&](uint32_t token) -> uint32_t & { return bins[token + token / kPer]; };
+
+    const int i = start + tid;
+    const Entry mine = i < N ? src.at(i) : Entry{0, 0};
+    for (int k = tid; k < kSmallBins + kSortThreads; k += kSortThreads) bins[k] = 0;
+    __syncthreads();
+    for (int k = 0; k < N; k += kRead * kSortThreads) {
+        uint32_t token[kRead];
+#pragma unroll
+        for (int j = 0; j < kRead; ++j) token[j] = src.at(min(k + j * kSortThreads + tid, N - 1)).token;
+#pragma unroll
+        for (int j = 0; j < kRead; ++j) {
+            const int at = k + j * kSortThreads;   // the workgroup's: a tile
+            if (at >= N) break;
+            const bool in = at + tid < N;
+            const uint32_t one = at < start ? 0x10001u : 1u;
+            // 64 alike (padding) at once: additions to one counter go one by one
+            if (__all(in && token[j] == __builtin_amdgcn_readfirstlane(token[j]))) {
+                if (lane == 0) atomicAdd(&bin(token[j]), kWave * one);
+            } else if (in) {
+                atomicAdd(&bin(token[j]), one);
+            }
+        }
+    }
+    __syncthreads();
+    uint32_t total = 0;
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) total += bins[tid * (kPer + 1) + j] & 0xffffu;
+    const uint32_t inc = wave_scan(total, lane);
+    if (lane == kWave - 1) sums[wave] = inc;
+    __syncthreads();
+    uint32_t below = lane < wave ? sums[lane] : 0;   // the waves' totals before this one's
+#pragma unroll
+    for (int off = kSortWaves / 2; off > 0; off >>= 1) below += __shfl_xor(below, off, kWave);
+    below = __builtin_amdgcn_readfirstlane(below) + inc - total;
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) {
+        const uint32_t c = bins[tid * (kPer + 1) + j];
+        bins[tid * (kPer + 1) + j] = below + (c >> 16);
+        below += c & 0xffffu;
+    }
+    const bool live = i < N;
+    uint64_t same = __ballot(live);   // the wave's lanes with this token
+#pragma unroll
+    for (int b = 0; b < 15; ++b) {
+        const uint64_t m = __ballot(mine.token >> b & 1);
+        same &= (mine.token >> b & 1) ? m : ~m;
+    }
+    for (int w = 0; w < kSortWaves; ++w) {
+        __syncthreads();
+        if (wave != w || !live) continue;
+        const uint32_t base = bin(mine.token);
+        out[base + __popcll(same & ((1ull << lane) - 1))] = mine;
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();   // every lane has read before the last of each token writes
+        if ((same >> lane) == 1) bin(mine.token) = base + __popcll(same);
+    }
+}
+
 // ---- the sums along the sorted order
 
 constexpr int kAhead = 8;   // rows of dout, or partial sums, in flight per wave
 
-// The first of the sorted entries lo .. N - 1 whose token is no less than t (N: none); the wave searches together, 65 ways a step.
+// The first of the sorted entries lo .. N - 1 whose token is no less than t (N: none); the wave searches
+// together, 65 ways a step.
 __device__ __forceinline__ int lower_bound(const Entry *e, int lo, int N, uint32_t t, int lane) {
     int hi = N;   // the answer is in [lo, hi]
     while (hi > lo) {
@@ -323,7 +404,8 @@ struct Sort {
     int N, V, D, chunk, chunks, pieces;   // chunk entries a wave, pieces vectors a row
 };
 
-// One wave per (chunk, strip of 64 vectors of columns). Runs of one token inside the chunk are
+// One wave per (chunk, strip of 64 vectors of columns); bound by the rows read and written: 16384 x 768
+// fp32 rows into 32000 25 us, 5.9 TB/s, with streaming loads and stores (28 with ordinary ones). Runs of one token inside the chunk are
 // written; a run that began before the chunk goes to partial[2 chunk], one that begins in it and
 // goes on behind it to partial[2 chunk + 1], both fp32.
 template <int DT>
@@ -527,7 +609,9 @@ inline int passes_of(int V) {   // the digits of 0 .. V
     while (bits < 31 && (static_cast<long long>(V) >> bits)) ++bits;
     return (bits + kBits - 1) / kBits;
 }
-inline int chunk_of(long long N) {   // about 1024 of them
+// About 1024 chunks, of at least 16 entries: shorter ones fill the device, longer ones leave less to join
+// (16384 x 768 fp32 rows of 32000 tokens 60, 62 and 80 us with 16, 64 and 128; 131072 240 with 8, 160 with 64).
+inline int chunk_of(long long N) {
     int c = 16;
     while (c < 512 && c * 1024LL < N) c *= 2;
     return c;
@@ -577,10 +661,11 @@ extern "C" int ulm_embed_fwd(const void *weight, int dtype, const long long *tok
     ULM_TRY(emb::check("ulm_embed_fwd", dtype, N, V, D));
     ULM_REQUIRE(weight && tokens && out, "ulm_embed_fwd: null pointer");
     const int vec = dtype == ULM_F32 ? 4 : 8, pieces = (D + vec - 1) / vec;
+    hipStream_t st = static_cast<hipStream_t>(stream);
     long long blocks = (N * pieces + emb::kThreads - 1) / emb::kThreads;
     if (blocks > 65536) blocks = 65536;
     emb::by_dtype(dtype, [&](auto dt) {
-        emb::fwd_kernel<decltype(dt)::value><<<dim3(static_cast<unsigned>(blocks)), dim3(emb::kThreads), 0, static_cast<hipStream_t>(stream)>>>(
+        emb::fwd_kernel<decltype(dt)::value><<<dim3(static_cast<unsigned>(blocks)), dim3(emb::kThreads), 0, st>>>(
             static_cast<const char *>(weight), tokens, static_cast<char *>(out), N, V, D, pieces, scale);
     });
     return check_launch("ulm_embed_fwd");
@@ -598,16 +683,25 @@ extern "C" int ulm_embed_bwd(const void *dout, int dtype, const long long *token
     const size_t need = ulm_embed_bwd_workspace_bytes(N, V, D);
     ULM_REQUIRE(workspace_bytes >= need, "ulm_embed_bwd: workspace %zu < %zu", workspace_bytes, need);
     const int chunks = emb::plan(nullptr, N, D).chunks;
-    const int vec = dtype == ULM_F32 ? 4 : 8, pieces = (D + vec - 1) / vec, strips = (pieces + kWave - 1) / kWave, W = emb::kThreads / kWave;
+    constexpr int W = emb::kThreads / kWave;
+    const int vec = dtype == ULM_F32 ? 4 : 8, pieces = (D + vec - 1) / vec, strips = (pieces + kWave - 1) / kWave;
     const long long sum_blocks = (static_cast<long long>(chunks) * strips + W - 1) / W;
     const long long zero_blocks = (static_cast<long long>(V) + W * emb::kZeroRows - 1) / (W * emb::kZeroRows);
     constexpr int JW = emb::kJoinThreads / kWave;
     const long long join_blocks = (static_cast<long long>(chunks) * strips + JW - 1) / JW;
-    ULM_REQUIRE(sum_blocks + zero_blocks < (1 << 24) && join_blocks < (1 << 23), "ulm_embed_bwd: N=%lld V=%d D=%d is too large", N, V, D);
+    ULM_REQUIRE(sum_blocks + zero_blocks < (1 << 24) && join_blocks < (1 << 23),
+                "ulm_embed_bwd: N=%lld V=%d D=%d is too large", N, V, D);
     const emb::Plan p = emb::plan(workspace, N, D);
     hipStream_t st = static_cast<hipStream_t>(stream);
-    const int n = static_cast<int>(N), passes = emb::passes_of(V);
+    const int n = static_cast<int>(N);
     emb::Source src{tokens, nullptr, V};
+    int passes = emb::passes_of(V);
+    if (N <= emb::kShort && V <= emb::kSmallV && passes > 1) {
+        const dim3 grid((n + emb::kSortThreads - 1) / emb::kSortThreads);
+        emb::place_small_kernel<<<grid, dim3(emb::kSortThreads), 0, st>>>(src, n, p.a);
+        src = {nullptr, p.a, V};
+        passes = 0;
+    }
     for (int k = 0; k < passes; ++k) {
         emb::Entry *to = k % 2 ? p.b : p.a;
         const int shift = k * emb::kBits;
@@ -626,7 +720,8 @@ extern "C" int ulm_embed_bwd(const void *dout, int dtype, const long long *token
     emb::by_dtype(dtype, [&](auto dt) {
         constexpr int DT = decltype(dt)::value;
         emb::sum_kernel<DT><<<dim3(static_cast<unsigned>(sum_blocks + zero_blocks)), dim3(emb::kThreads), 0, st>>>(
-            s, static_cast<const char *>(dout), static_cast<char *>(dweight), p.partial, scale, strips, static_cast<int>(sum_blocks));
+            s, static_cast<const char *>(dout), static_cast<char *>(dweight), p.partial, scale, strips,
+            static_cast<int>(sum_blocks));
         if (p.chunks > 1)
             emb::join_kernel<DT><<<dim3(static_cast<unsigned>(join_blocks)), dim3(emb::kJoinThreads), 0, st>>>(
                 s, static_cast<char *>(dweight), p.partial, scale, strips);
