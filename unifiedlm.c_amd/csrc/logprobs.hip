@@ -28,7 +28,9 @@ constexpr float kHuge = 0x1p96f;      // maxima beyond which m log2(e) is not fo
 typedef uint32_t u32x4_any __attribute__((vector_size(16), aligned(2)));   // rows may start anywhere
 
 // 16 bytes of a stream that the caches need not keep (bf16 rows of 32000: 6.7 TB/s, 5.9 with ordinary loads)
-__device__ __forceinline__ u32x4_any load_once(const char *p) { return __builtin_nontemporal_load(reinterpret_cast<const u32x4_any *>(p)); }
+__device__ __forceinline__ u32x4_any load_once(const char *p) {
+    return __builtin_nontemporal_load(reinterpret_cast<const u32x4_any *>(p));
+}
 
 template <int DT> struct Elem { static constexpr int vec = DT == ULM_F32 ? 4 : 8, bytes = DT == ULM_F32 ? 4 : 2; };
 
@@ -115,8 +117,9 @@ template <int W> __device__ __forceinline__ Sums group_add(Sums v) {
 }
 
 // A thread's running sums in powers of two about ref = m log2(e), rounded: s = sum 2^t_i,
-// u = sum 2^t_i t_i with t_i = x_i log2(e) - ref in one fused operation (6 instructions an
-// element, conversion and maximum included, where differences from m itself take 8). What ref
+// u = sum 2^t_i t_i with t_i = x_i log2(e) - ref in one fused operation (5.5 instructions an
+// element, conversion and maximum included, where differences from m itself and a guard for
+// masked ones take 8: at 16384 rows of 32000 bf16 the ALUs were busy 83% of 204 us). What ref
 // lacks of m log2(e) is put right at the end. Where |m| is so large that ref could
 // overflow (rows masked with the type's lowest value), t_i = (x_i - m) log2(e).
 struct Running {
@@ -375,7 +378,9 @@ template <int N> __device__ __forceinline__ float take(const float (&x)[N], bool
 }
 
 // One workgroup of NT threads per (row, part). With one part it writes the row's outputs, with
-// more the part's sums and its `top` best keys in order (0 where it has fewer).
+// more the part's sums and its `top` best keys in order (0 where it has fewer). One pass over the
+// row, which bounds it: 16384 rows of 32000 bf16 157 us, 6.7 TB/s. Workgroups that go from row to row with the
+// next loads ahead took 197 (118 registers leave half the waves), the alternatives 30 more.
 template <int DT, bool TOP, int NT>
 __global__ __launch_bounds__(NT) void fwd_kernel(Rows a, Outs o, Sums *part_sums, uint64_t *part_keys) {
     using T = Tile<DT, NT>;
@@ -411,7 +416,8 @@ __global__ __launch_bounds__(NT) void fwd_kernel(Rows a, Outs o, Sums *part_sums
             }
         } else {
 #pragma unroll
-            for (int j = 0; j < kUnroll; ++j) load_vec<DT>(row, T::at(e0, k, j, tid), e1, *reinterpret_cast<float(*)[V]>(&x[j * V]));
+            for (int j = 0; j < kUnroll; ++j)
+                load_vec<DT>(row, T::at(e0, k, j, tid), e1, *reinterpret_cast<float(*)[V]>(&x[j * V]));
         }
         const float most = take(x, !whole, masked, v);
         if constexpr (TOP) scratch.table[k * NT + tid] = v.s == v.s ? most : __uint_as_float(0x7fc00000u);
@@ -480,62 +486,78 @@ struct Grads {
     char *dx;   // (rows, V), dense
 };
 
-// One workgroup per (row, tile): a vector a thread. At 16384 x 32000 in bf16 338 us, 6.2 TB/s, with
-// stores that leave the caches to others; 404 with ordinary ones, 357 and 360 with two and four
-// vectors a thread.
-template <int DT, bool ENT>
+// One workgroup per (row, tile of U vectors a thread). At 16384 x 32000 in bf16 341 us, 6.2 TB/s, with one
+// vector a thread and stores that leave the caches to others; 404 with ordinary stores, 357 and 360
+// with two and four vectors. With alternatives a workgroup has more to do besides (their gradients' sum,
+// their elements), and two vectors share it: 16384 x 32000 in bf16 with 5 of them and the entropy 381 us,
+// 464 with one (364 with four, but 90 instead of 85 at 2048 x 32000 in fp32 with 20).
+template <int DT, bool ENT, int U>
 __global__ __launch_bounds__(kThreads) void bwd_kernel(Rows a, Grads g, int tiles) {
-    constexpr int V = Elem<DT>::vec, kTile = kThreads * V, B = Elem<DT>::bytes;
+    constexpr int V = Elem<DT>::vec, kTile = kThreads * V * U, B = Elem<DT>::bytes;
     const long long id = block_id(), r = id / tiles;
     if (r >= a.rows) return;
-    const int tid = threadIdx.x, e0 = static_cast<int>(id - r * tiles) * kTile, e1 = min(a.V, e0 + kTile), i = e0 + tid * V;
+    const int tid = threadIdx.x, lane = tid % kWave;
+    const int e0 = static_cast<int>(id - r * tiles) * kTile, e1 = min(a.V, e0 + kTile);
     const char *row = a.row(r, B);
     char *out = g.dx + static_cast<size_t>(r) * a.V * B;
-    float x[V];
-    if (i < e1) load_vec<DT>(row, i, e1, x);
-
+    // the row's numbers first: they arrive while its elements are under way
     const float m = g.stats[2 * r], logs = g.stats[2 * r + 1];
     const float h = ENT ? g.dentropy[r] : 0.f, H = ENT ? g.entropy[r] : 0.f;
     const long long t = a.tokens[r];
-    float da = g.dlogprob && t != a.ignore ? g.dlogprob[r] : 0.f;
+    const float dl = g.dlogprob ? g.dlogprob[r] : 0.f;
+    float x[U][V];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        const int i = e0 + (u * kThreads + tid) * V;
+        if (i < e1) load_vec<DT>(row, i, e1, x[u]);
+    }
+
+    float da = t != a.ignore ? dl : 0.f;
     if (t != a.ignore && (t < 0 || t >= a.V)) da = __uint_as_float(0x7fc00000u);
-    float G = da;
-    if (g.dtop)
-        for (int j = 0; j < a.top; ++j) G += g.dtop[r * a.top + j];
+    float G = da, dc = 0.f;
+    long long which = -1;   // lane's alternative, and its gradient
+    if (g.dtop) {
+        if (lane < a.top) {
+            dc = g.dtop[r * a.top + lane];
+            which = g.top_tokens[r * a.top + lane];
+        }
+        G += wave_sum(dc);
+    }
     const bool empty = m == -INFINITY && logs == -INFINITY;
     auto grad = [&](float x) {   // without the tokens' own terms
         const float d = x - m, p = exp_of(d - logs);
         const float f = ENT ? __builtin_fmaf(h, (fmaxf(d, kFloor) - logs) + H, G) : G;
         return empty ? 0.f : -p * f;
     };
-    if (i < e1) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        const int i = e0 + (u * kThreads + tid) * V;
+        if (i >= e1) continue;
         const long long own = t - i;   // the token's place among these
 #pragma unroll
         for (int k = 0; k < V; ++k) {
-            x[k] = grad(x[k]);
-            if (own == k && !empty) x[k] += da;
+            x[u][k] = grad(x[u][k]);
+            if (own == k && !empty) x[u][k] += da;
         }
         if (i + V <= e1) {
             u32x4_any w;
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
-                if constexpr (DT == ULM_F32) w[k] = __float_as_uint(x[k]);
-                else w[k] = pack_word<DT>(x[2 * k], x[2 * k + 1]);
+                if constexpr (DT == ULM_F32) w[k] = __float_as_uint(x[u][k]);
+                else w[k] = pack_word<DT>(x[u][2 * k], x[u][2 * k + 1]);
             }
             __builtin_nontemporal_store(w, reinterpret_cast<u32x4_any *>(out + static_cast<size_t>(i) * B));
         } else {
 #pragma unroll
             for (int k = 0; k < V; ++k)
-                if (i + k < e1) store_from_f32(out, i + k, DT, x[k]);
+                if (i + k < e1) store_from_f32(out, i + k, DT, x[u][k]);
         }
     }
     if (!g.dtop || empty) return;
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // the streaming stores are done
     __syncthreads();   // the alternatives' elements are written again, with their own terms
-    if (tid < a.top) {
-        const long long j = g.top_tokens[r * a.top + tid];
-        if (j >= e0 && j < e1)
-            store_from_f32(out, j, DT, grad(load_as_f32(row, j, DT)) + g.dtop[r * a.top + tid] + (j == t ? da : 0.f));
-    }
+    if (tid < a.top && which >= e0 && which < e1)
+        store_from_f32(out, which, DT, grad(load_as_f32(row, which, DT)) + dc + (which == t ? da : 0.f));
 }
 
 // How the rows are spread: a function of the sizes, the same for the workspace and the launch. A
@@ -569,7 +591,8 @@ using namespace ulm;
 static int check_rows(const char *fn, long long rows, long long inner, int V, int top, int dtype) {
     if (rows < 1 || rows > (1LL << 34) || inner < 1 || V < 1 || V > (1 << 30))
         return fail(ULM_ERR_INVALID, "%s: bad sizes rows=%lld inner=%lld V=%d", fn, rows, inner, V);
-    if (top < 0 || top > lp::kMaxTop || top > V) return fail(ULM_ERR_INVALID, "%s: top=%d outside 0 .. min(V, %d)", fn, top, lp::kMaxTop);
+    if (top < 0 || top > lp::kMaxTop || top > V)
+        return fail(ULM_ERR_INVALID, "%s: top=%d outside 0 .. min(V, %d)", fn, top, lp::kMaxTop);
     if (top && V > lp::kMaxTopV) return fail(ULM_ERR_INVALID, "%s: top=%d with V=%d", fn, top, V);
     if (!valid_dtype(dtype)) return fail(ULM_ERR_INVALID, "%s: bad dtype %d", fn, dtype);
     return ULM_OK;
@@ -597,11 +620,13 @@ extern "C" int ulm_token_logprobs(const void *logits, int dtype, const long long
     const lp::Plan plan = lp::plan_of(rows, V, top, dtype);
     const int parts = plan.parts;
     const size_t need = ulm_token_logprobs_workspace_bytes(rows, V, top, dtype);
-    ULM_REQUIRE(workspace_bytes >= need && (need == 0 || workspace), "ulm_token_logprobs: workspace %zu < %zu", workspace_bytes, need);
+    ULM_REQUIRE(workspace_bytes >= need && (need == 0 || workspace), "ulm_token_logprobs: workspace %zu < %zu",
+                workspace_bytes, need);
     Carver c(workspace);
     lp::Sums *sums = parts > 1 ? c.take<lp::Sums>(static_cast<size_t>(rows) * parts) : nullptr;
     uint64_t *keys = parts > 1 ? c.take<uint64_t>(static_cast<size_t>(rows) * parts * top) : nullptr;
-    const lp::Rows a{static_cast<const char *>(logits), tokens, inner, outer_stride, row_stride, ignore_index, rows, V, top, parts, plan.part_len};
+    const lp::Rows a{static_cast<const char *>(logits), tokens, inner, outer_stride, row_stride, ignore_index, rows, V, top,
+                     parts, plan.part_len};
     const lp::Outs o{logprob, entropy, top_logprobs, stats, top_tokens};
     hipStream_t s = static_cast<hipStream_t>(stream);
     auto launch = [&](auto dt, auto with_top) {
@@ -634,15 +659,22 @@ extern "C" int ulm_token_logprobs_bwd(const void *logits, int dtype, const long 
     ULM_REQUIRE(logits && tokens && stats && dlogits && (!dentropy || entropy) && (!dtop || (top_tokens && top)),
                 "ulm_token_logprobs_bwd: null pointer");
     ULM_REQUIRE(dlogits != logits, "ulm_token_logprobs_bwd: dlogits must not alias logits");
-    const int tile = lp::kThreads * (dtype == ULM_F32 ? 4 : 8), tiles = (V + tile - 1) / tile;
-    const lp::Rows a{static_cast<const char *>(logits), tokens, inner, outer_stride, row_stride, ignore_index, rows, V, top, 1, V};
+    const int each = dtop ? 2 : 1;   // vectors a thread
+    const int tile = lp::kThreads * each * (dtype == ULM_F32 ? 4 : 8), tiles = (V + tile - 1) / tile;
+    const lp::Rows a{static_cast<const char *>(logits), tokens, inner, outer_stride, row_stride, ignore_index, rows, V, top,
+                     1, V};
     const lp::Grads g{stats, entropy, dlogprob, dentropy, dtop, top_tokens, static_cast<char *>(dlogits)};
     hipStream_t s = static_cast<hipStream_t>(stream);
     const dim3 grid = lp::grid_of(rows * tiles), block(lp::kThreads);
     auto launch = [&](auto dt) {
         constexpr int DT = decltype(dt)::value;
-        if (dentropy) lp::bwd_kernel<DT, true><<<grid, block, 0, s>>>(a, g, tiles);
-        else lp::bwd_kernel<DT, false><<<grid, block, 0, s>>>(a, g, tiles);
+        if (each == 2) {
+            if (dentropy) lp::bwd_kernel<DT, true, 2><<<grid, block, 0, s>>>(a, g, tiles);
+            else lp::bwd_kernel<DT, false, 2><<<grid, block, 0, s>>>(a, g, tiles);
+        } else {
+            if (dentropy) lp::bwd_kernel<DT, true, 1><<<grid, block, 0, s>>>(a, g, tiles);
+            else lp::bwd_kernel<DT, false, 1><<<grid, block, 0, s>>>(a, g, tiles);
+        }
     };
     if (dtype == ULM_F32) launch(std::integral_constant<int, ULM_F32>{});
     else if (dtype == ULM_BF16) launch(std::integral_constant<int, ULM_BF16>{});
