@@ -580,10 +580,12 @@ void check_capture(const Tensor &leaf) {
     if (!leaf.requires_grad() || !leaf.is_leaf() || !at::GradMode::is_enabled()) return;
     hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
     const auto now = c10::hip::getCurrentHIPStream(leaf.get_device());
-    if (hipStreamIsCapturing(now.stream(), &status) != hipSuccess || status == hipStreamCaptureStatusNone) return;
+    if (hipStreamIsCapturing(now.stream(), &status) != hipSuccess) (void)hipGetLastError();   // not this call's to report
+    if (status == hipStreamCaptureStatusNone) return;
     const auto node = torch::autograd::impl::try_get_grad_accumulator(leaf);
     TORCH_CHECK(!node || !node->stream() || node->stream()->id() == now.id(),
-                "captured while an eager graph of the same leaf is alive on another stream: let go of that graph's outputs first");
+                "captured while an eager graph of the same leaf is alive on another stream: let go of "
+                "that graph's outputs first");
 }
 
 struct TokenLogprobs : torch::autograd::Function<TokenLogprobs> {
@@ -634,8 +636,8 @@ struct TokenLogprobs : torch::autograd::Function<TokenLogprobs> {
             using F = Tensor(const Tensor &, const Tensor &, c10::SymInt, c10::SymInt, const Tensor &, const Tensor &,
                              const Tensor &, O, O, O);
             auto opt = [](const Tensor &t) { return t.defined() ? std::optional<Tensor>(t) : std::nullopt; };
-            out[0] = registered<F>("ulm::token_logprobs_bwd").call(logits, tokens, top, ignore, stats, entropy, top_tok, opt(grads[0]),
-                                                                   opt(grads[1]), opt(grads[2]));
+            out[0] = registered<F>("ulm::token_logprobs_bwd").call(logits, tokens, top, ignore, stats, entropy, top_tok,
+                                                                   opt(grads[0]), opt(grads[1]), opt(grads[2]));
             return out;
         }
         at::AutoDispatchBelowAutograd guard;
@@ -649,16 +651,17 @@ struct TokenLogprobs : torch::autograd::Function<TokenLogprobs> {
         for (int i = 0; i < 3; ++i)
             if (grads[i].defined() && grads[i].numel()) up[i] = f32c(grads[i]);
         check("ulm_token_logprobs_bwd",
-              ulm_token_logprobs_bwd(r.x.data_ptr(), code(logits.scalar_type()), ip(tok), r.rows, r.inner, r.outer_stride, r.row_stride,
-                                     r.V, top, ignore, fp(st), fp(H), ip(tt), fp(up[0]), fp(up[1]), fp(up[2]), out[0].data_ptr(),
-                                     stream_of(logits)));
+              ulm_token_logprobs_bwd(r.x.data_ptr(), code(logits.scalar_type()), ip(tok), r.rows, r.inner, r.outer_stride,
+                                     r.row_stride, r.V, top, ignore, fp(st), fp(H), ip(tt), fp(up[0]), fp(up[1]),
+                                     fp(up[2]), out[0].data_ptr(), stream_of(logits)));
         return out;
     }
 };
 
 bool wants_grad(const Tensor &t) { return t.requires_grad() && at::GradMode::is_enabled(); }
 
-py::object token_logprobs(const py::handle &logits_, const py::handle &tokens_, const py::handle &top_, const py::handle &ignore_) {
+py::object token_logprobs(const py::handle &logits_, const py::handle &tokens_, const py::handle &top_,
+                          const py::handle &ignore_) {
     if (!plain_thread() || !PyLong_CheckExact(top_.ptr()) || !PyLong_CheckExact(ignore_.ptr())) return py::none();
     const Tensor logits = plain(logits_), tokens = plain_ids(tokens_);
     if (!logits.defined() || !tokens.defined() || !has_code(logits) || logits.device() != tokens.device() || logits.dim() < 1 ||
@@ -718,8 +721,8 @@ struct Embedding : torch::autograd::Function<Embedding> {
         const Tensor dw = make({V, D}, dt);
         const size_t wb = ulm_embed_bwd_workspace_bytes(N, V, D);
         const Tensor ws = make.bytes(wb);
-        check("ulm_embed_bwd", ulm_embed_bwd(dout.data_ptr(), code(dt), ip(tok), N, V, D, static_cast<float>(scale), dw.data_ptr(),
-                                             ws.data_ptr(), wb, stream_of(dout)));
+        check("ulm_embed_bwd", ulm_embed_bwd(dout.data_ptr(), code(dt), ip(tok), N, V, D, static_cast<float>(scale),
+                                             dw.data_ptr(), ws.data_ptr(), wb, stream_of(dout)));
         return {dw, Tensor(), Tensor()};
     }
 };
@@ -772,7 +775,8 @@ Tensor run_norm(const std::vector<ulm_grad> &table, const Tensor &like, int norm
     const size_t wb = ulm_grad_norm_workspace_bytes(table.data(), table.size());
     const Tensor ws = make.bytes(wb);
     if (bound)
-        check("ulm_clip_grads", ulm_clip_grads(table.data(), table.size(), norm, *bound, fpm(out), ws.data_ptr(), wb, stream_of(like)));
+        check("ulm_clip_grads", ulm_clip_grads(table.data(), table.size(), norm, *bound, fpm(out), ws.data_ptr(), wb,
+                                               stream_of(like)));
     else
         check("ulm_grad_norm", ulm_grad_norm(table.data(), table.size(), norm, fpm(out), ws.data_ptr(), wb, stream_of(like)));
     return out;
@@ -831,12 +835,14 @@ Tensor clip(const std::vector<Tensor> &grads, const std::vector<Tensor> &out, do
 py::object clip_grads(const py::handle &grads_, const py::handle &max_norm, const py::handle &out_, const py::handle &norm_type) {
     std::vector<Tensor> grads, out;
     const int norm = norm_code(norm_type);
-    if (!plain_thread() || norm < 0 || !(PyFloat_CheckExact(max_norm.ptr()) || PyLong_CheckExact(max_norm.ptr()))) return py::none();
+    if (!plain_thread() || norm < 0 || !(PyFloat_CheckExact(max_norm.ptr()) || PyLong_CheckExact(max_norm.ptr())))
+        return py::none();
     const double bound = max_norm.cast<double>();
     if (!(bound >= 0) || !plain_list(grads_, grads)) return py::none();
     const bool fresh = out_.is_none();
     if (out_.ptr() == grads_.ptr()) out = grads;
-    else if (!fresh && (!plain_list(out_, out) || out.size() != grads.size() || out[0].device() != grads[0].device())) return py::none();
+    else if (!fresh && (!plain_list(out_, out) || out.size() != grads.size() || out[0].device() != grads[0].device()))
+        return py::none();
     const Tensor n = unlocked([&] {
         if (fresh)
             for (const Tensor &g : grads) {
