@@ -279,6 +279,21 @@ def test_views(view, dt):
         assert all(torch.equal(s, t) for s, t in zip(a, b))
 
 
+@pytest.mark.parametrize("dt", ["fp32", "bf16"])
+@pytest.mark.parametrize("shape", [(3, 5), (2, 3, 4), (600, 2)])
+def test_rows_repeated_over_a_leading_dimension(shape, dt):
+    """One block of rows expanded in front: the rows' outer stride is 0."""
+    say(f"token_logprobs expanded leading dimension {shape} {dt}")
+    gen = torch.Generator().manual_seed(43)
+    V = 333
+    x = (torch.randn(1, *shape[1:], V, generator=gen) * 2).to(DT[dt]).cuda().expand(*shape, V)
+    assert x.stride(0) == 0
+    tokens = torch.randint(0, V, shape, generator=gen).cuda()
+    check(x, tokens, 3, up=ups(gen, shape, 3))
+    a, b = kernel.token_logprobs(x, tokens, 3), kernel.token_logprobs(x.contiguous(), tokens, 3)
+    assert all(torch.equal(s, t) for s, t in zip(a, b))
+
+
 def test_a_row_does_not_depend_on_the_others():
     """Equal bits however many rows come along, as long as they take workgroups of one size (more than 512 rows)."""
     say("token_logprobs rows alone")

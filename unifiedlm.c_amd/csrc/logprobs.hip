@@ -153,7 +153,7 @@ struct Rows {
     long long ignore, rows;
     int V, top, parts, part_len;
     __device__ __forceinline__ const char *row(long long r, int bytes) const {
-        const long long outer = outer_stride ? r / inner : 0;
+        const long long outer = r < inner ? 0 : r / inner;   // mostly one stride: no division
         return x + (outer * outer_stride + (r - outer * inner) * row_stride) * bytes;
     }
 };
