@@ -7,6 +7,7 @@
 // positions by a stable radix sort, the rows of dout are summed along the sorted order in
 // chunks of equal length, one wave each, and sums that go over a chunk's end are
 // joined afterwards. No atomics on numbers: equal inputs give equal bits.
+#include <algorithm>
 #include <type_traits>
 
 #include "ulm_common.h"
@@ -221,18 +222,45 @@ __global__ __launch_bounds__(kWave) void scan_kernel(uint32_t *counts, int tiles
     if (lane == 0) totals[blockIdx.x] = before;
 }
 
+// dW as zeros, by the workgroups behind a short sequence's first sorting launch: the sort leaves most of the
+// device idle, and the rows that occur are written over by their sums. 16384 x 768 fp32 rows into 32000: the
+// gradient 38 us, 46 with only the absent rows zeroed, beside the sums; of one token 19 and 26. Ordinary stores
+// take 40, more of them a thread 40 (four, eight).
+struct Zero {
+    static constexpr int kStores = 2, kBytes = kStores * kSortThreads * 16;   // a workgroup's at a time
+    char *dw;
+    size_t bytes;
+    int from;   // the first workgroup
+    __device__ __forceinline__ bool take(int tid) const {
+        if (static_cast<int>(blockIdx.x) < from) return false;
+        const size_t step = static_cast<size_t>(gridDim.x - from) * kBytes;
+        for (size_t at = static_cast<size_t>(blockIdx.x - from) * kBytes; at < bytes; at += step) {
+#pragma unroll
+            for (int j = 0; j < kStores; ++j) {
+                const size_t b = at + (j * kSortThreads + tid) * 16;
+                if (b + 16 <= bytes) __builtin_nontemporal_store(u32x4_any{0, 0, 0, 0}, reinterpret_cast<u32x4_any *>(dw + b));
+                else
+                    for (size_t k = b; k < bytes; k += 2) *reinterpret_cast<uint16_t *>(dw + k) = 0;
+            }
+        }
+        return true;
+    }
+    unsigned blocks() const { return static_cast<unsigned>(std::min<size_t>((bytes + kBytes - 1) / kBytes, 1 << 16)); }
+};
+
 // Every entry of a tile of PER x kSortThreads to its place: the smaller digits' total, the same
 // digit's entries in earlier tiles, in earlier waves of this tile, and among the lanes before.
 // COUNT: the first two are counted here, by every workgroup, over the whole sequence, which for
 // a short one takes less time than two more launches (counts and totals are not used then).
 template <int PER, bool COUNT>
 __global__ __launch_bounds__(kSortThreads) void place_kernel(Source src, int N, int shift, const uint32_t *counts, int tiles,
-                                                             const uint32_t *totals, Entry *out) {
+                                                             const uint32_t *totals, Entry *out, Zero zero) {
     static_assert(kBins == kSortThreads, "one bin per thread");
     __shared__ uint32_t base[kBins], all[COUNT ? kBins : 1];
     __shared__ uint16_t seen[kSortWaves][kBins];   // a wave's entries of each digit, then those of the waves before it
     __shared__ uint32_t sums[kSortWaves];
     const int tid = threadIdx.x, lane = tid % kWave, wave = tid / kWave, tile = blockIdx.x, start = tile * PER * kSortThreads;
+    if (COUNT && zero.take(tid)) return;
 
     Entry e[PER];
 #pragma unroll
@@ -313,19 +341,24 @@ __global__ __launch_bounds__(kSortThreads) void place_kernel(Source src, int N, 
 
 // The whole sort of a short sequence of tokens below kSmallV in one launch: every workgroup
 // counts all tokens, those of earlier tiles in the counter's upper half, turns the counts
-// into the places where its tile's entries begin, and its waves take theirs in turn. At 16384 tokens 12 us,
-// where the two digits' launches take 18 (the whole gradient 47 and 54, at 32768 47 and 58).
+// into the places where its tile's entries begin, and its tile's waves take theirs in turn. At 16384
+// tokens 13 us, where the two digits' launches take 20; with tiles of 1024 entries, 16 turns, 1 us more, of
+// 128 as long as with 256.
+constexpr int kSmallTile = 256;
 constexpr int kSmallV = (1 << 15) - 1;   // tokens 0 .. kSmallV, the last one for those outside
-__global__ __launch_bounds__(kSortThreads) void place_small_kernel(Source src, int N, Entry *out) {
+__global__ __launch_bounds__(kSortThreads) void place_small_kernel(Source src, int N, Entry *out, Zero zero) {
     constexpr int kSmallBins = kSmallV + 1, kPer = kSmallBins / kSortThreads, kRead = 16;
-    __shared__ uint32_t bins[kSmallBins + kSortThreads];   // a word between threads' shares, off the same bank
+    alignas(16) __shared__ uint32_t bins[kSmallBins + kSortThreads];   // a word between threads' shares, off the same bank
     __shared__ uint32_t sums[kSortWaves];
-    const int tid = threadIdx.x, lane = tid % kWave, wave = tid / kWave, start = blockIdx.x * kSortThreads;
+    const int tid = threadIdx.x, lane = tid % kWave, wave = tid / kWave, start = blockIdx.x * kSmallTile;
     auto bin = [&](uint32_t token) -> uint32_t & { return bins[token + token / kPer]; };
 
+    if (zero.take(tid)) return;
     const int i = start + tid;
-    const Entry mine = i < N ? src.at(i) : Entry{0, 0};
-    for (int k = tid; k < kSmallBins + kSortThreads; k += kSortThreads) bins[k] = 0;
+    const bool live = tid < kSmallTile && i < N;
+    const Entry mine = live ? src.at(i) : Entry{0, 0};
+    for (int k = 4 * tid; k < kSmallBins + kSortThreads; k += 4 * kSortThreads)
+        *reinterpret_cast<uint4 *>(&bins[k]) = uint4{0, 0, 0, 0};
     __syncthreads();
     for (int k = 0; k < N; k += kRead * kSortThreads) {
         uint32_t token[kRead];
@@ -333,10 +366,10 @@ __global__ __launch_bounds__(kSortThreads) void place_small_kernel(Source src, i
         for (int j = 0; j < kRead; ++j) token[j] = src.at(min(k + j * kSortThreads + tid, N - 1)).token;
 #pragma unroll
         for (int j = 0; j < kRead; ++j) {
-            const int at = k + j * kSortThreads;   // the workgroup's: a tile
+            const int at = k + j * kSortThreads;
             if (at >= N) break;
             const bool in = at + tid < N;
-            const uint32_t one = at < start ? 0x10001u : 1u;
+            const uint32_t one = at + wave * kWave < start ? 0x10001u : 1u;   // the wave's: in one tile
             // 64 alike (padding) at once: additions to one counter go one by one
             if (__all(in && token[j] == __builtin_amdgcn_readfirstlane(token[j]))) {
                 if (lane == 0) atomicAdd(&bin(token[j]), kWave * one);
@@ -362,14 +395,13 @@ __global__ __launch_bounds__(kSortThreads) void place_small_kernel(Source src, i
         bins[tid * (kPer + 1) + j] = below + (c >> 16);
         below += c & 0xffffu;
     }
-    const bool live = i < N;
     uint64_t same = __ballot(live);   // the wave's lanes with this token
 #pragma unroll
     for (int b = 0; b < 15; ++b) {
         const uint64_t m = __ballot(mine.token >> b & 1);
         same &= (mine.token >> b & 1) ? m : ~m;
     }
-    for (int w = 0; w < kSortWaves; ++w) {
+    for (int w = 0; w < kSmallTile / kWave; ++w) {
         __syncthreads();
         if (wave != w || !live) continue;
         const uint32_t base = bin(mine.token);
@@ -405,9 +437,9 @@ struct Sort {
 };
 
 // One wave per (chunk, strip of 64 vectors of columns); bound by the rows read and written: 16384 x 768
-// fp32 rows into 32000 25 us, 5.9 TB/s, with streaming loads and stores (28 with ordinary ones). Runs of one token inside the chunk are
-// written; a run that began before the chunk goes to partial[2 chunk], one that begins in it and
-// goes on behind it to partial[2 chunk + 1], both fp32.
+// fp32 rows into 32000 13 us, 5.6 TB/s; streaming loads and stores take a tenth less than ordinary ones. Runs of
+// one token inside the chunk are written; a run that began before the chunk goes to partial[2 chunk],
+// one that begins in it and goes on behind it to partial[2 chunk + 1], both fp32.
 template <int DT>
 __device__ __forceinline__ void sum_chunk(const Sort &s, const char *dout, char *dw, float *partial, float scale, int chunk,
                                           int strip, int lane) {
@@ -476,7 +508,7 @@ __device__ __forceinline__ void sum_chunk(const Sort &s, const char *dout, char 
     else put_row();
 }
 
-constexpr int kZeroRows = 8;   // rows of dW a wave looks after: the absent ones are zeroed
+constexpr int kZeroRows = 8;   // rows of dW a wave looks after behind a long sequence's sums: the absent ones are zeroed
 
 template <int DT>
 __global__ __launch_bounds__(kThreads) void sum_kernel(Sort s, const char *dout, char *dw, float *partial, float scale,
@@ -686,7 +718,8 @@ extern "C" int ulm_embed_bwd(const void *dout, int dtype, const long long *token
     constexpr int W = emb::kThreads / kWave;
     const int vec = dtype == ULM_F32 ? 4 : 8, pieces = (D + vec - 1) / vec, strips = (pieces + kWave - 1) / kWave;
     const long long sum_blocks = (static_cast<long long>(chunks) * strips + W - 1) / W;
-    const long long zero_blocks = (static_cast<long long>(V) + W * emb::kZeroRows - 1) / (W * emb::kZeroRows);
+    const bool few = N <= emb::kShort;
+    const long long zero_blocks = few ? 0 : (static_cast<long long>(V) + W * emb::kZeroRows - 1) / (W * emb::kZeroRows);
     constexpr int JW = emb::kJoinThreads / kWave;
     const long long join_blocks = (static_cast<long long>(chunks) * strips + JW - 1) / JW;
     ULM_REQUIRE(sum_blocks + zero_blocks < (1 << 24) && join_blocks < (1 << 23),
@@ -696,23 +729,26 @@ extern "C" int ulm_embed_bwd(const void *dout, int dtype, const long long *token
     const int n = static_cast<int>(N);
     emb::Source src{tokens, nullptr, V};
     int passes = emb::passes_of(V);
-    if (N <= emb::kShort && V <= emb::kSmallV && passes > 1) {
-        const dim3 grid((n + emb::kSortThreads - 1) / emb::kSortThreads);
-        emb::place_small_kernel<<<grid, dim3(emb::kSortThreads), 0, st>>>(src, n, p.a);
+    emb::Zero zero{static_cast<char *>(dweight), static_cast<size_t>(V) * D * (dtype == ULM_F32 ? 4 : 2), 0};
+    if (few && V <= emb::kSmallV && passes > 1) {
+        zero.from = (n + emb::kSmallTile - 1) / emb::kSmallTile;
+        const dim3 grid(zero.from + zero.blocks());
+        emb::place_small_kernel<<<grid, dim3(emb::kSortThreads), 0, st>>>(src, n, p.a, zero);
         src = {nullptr, p.a, V};
         passes = 0;
     }
     for (int k = 0; k < passes; ++k) {
         emb::Entry *to = k % 2 ? p.b : p.a;
         const int shift = k * emb::kBits;
-        if (N <= emb::kShort) {
-            const dim3 grid((n + emb::kSortThreads - 1) / emb::kSortThreads);
-            emb::place_kernel<1, true><<<grid, dim3(emb::kSortThreads), 0, st>>>(src, n, shift, nullptr, 0, nullptr, to);
+        if (few) {
+            zero.from = (n + emb::kSortThreads - 1) / emb::kSortThreads;
+            const dim3 grid(zero.from + (k ? 0 : zero.blocks()));
+            emb::place_kernel<1, true><<<grid, dim3(emb::kSortThreads), 0, st>>>(src, n, shift, nullptr, 0, nullptr, to, zero);
         } else {
             emb::count_kernel<<<dim3(p.tiles), dim3(emb::kSortThreads), 0, st>>>(src, n, shift, p.counts, p.tiles);
             emb::scan_kernel<<<dim3(emb::kBins), dim3(kWave), 0, st>>>(p.counts, p.tiles, p.totals);
             emb::place_kernel<emb::kTile / emb::kSortThreads, false><<<dim3(p.tiles), dim3(emb::kSortThreads), 0, st>>>(
-                src, n, shift, p.counts, p.tiles, p.totals, to);
+                src, n, shift, p.counts, p.tiles, p.totals, to, zero);
         }
         src = {nullptr, to, V};
     }
