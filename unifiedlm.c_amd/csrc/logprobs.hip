@@ -486,16 +486,18 @@ struct Grads {
     char *dx;   // (rows, V), dense
 };
 
-// One workgroup per (row, tile of U vectors a thread). At 16384 x 32000 in bf16 341 us, 6.2 TB/s, with one
+// One workgroup per (row, tile of U vectors a thread). At 16384 x 32000 in bf16 340 us, 6.2 TB/s, with one
 // vector a thread and stores that leave the caches to others; 404 with ordinary stores, 357 and 360
 // with two and four vectors. With alternatives a workgroup has more to do besides (their gradients' sum,
 // their elements), and two vectors share it: 16384 x 32000 in bf16 with 5 of them and the entropy 381 us,
-// 464 with one (364 with four, but 90 instead of 85 at 2048 x 32000 in fp32 with 20).
+// 464 with one (364 with four, but 90 instead of 85 at 2048 x 32000 in fp32 with 20). From the last row
+// back: the caches still hold what the forward read last (1% of the pair from 2048 to 16384 rows).
 template <int DT, bool ENT, int U>
 __global__ __launch_bounds__(kThreads) void bwd_kernel(Rows a, Grads g, int tiles) {
     constexpr int V = Elem<DT>::vec, kTile = kThreads * V * U, B = Elem<DT>::bytes;
-    const long long id = block_id(), r = id / tiles;
-    if (r >= a.rows) return;
+    const long long id = a.rows * tiles - 1 - block_id();
+    if (id < 0) return;
+    const long long r = id / tiles;
     const int tid = threadIdx.x, lane = tid % kWave;
     const int e0 = static_cast<int>(id - r * tiles) * kTile, e1 = min(a.V, e0 + kTile);
     const char *row = a.row(r, B);
