@@ -304,6 +304,25 @@ def test_a_row_does_not_depend_on_the_others():
     assert all(torch.equal(s, t) for s, t in zip(a, c))
 
 
+@pytest.mark.parametrize("dt", ["fp32", "bf16"])
+def test_more_rows_than_one_grid_dimension_counts(dt):
+    """2^20 + 1537 rows, a block of 1024 over and over: every copy has the first one's bits, its gradients too."""
+    say(f"token_logprobs rows past 2^20 {dt}")
+    rows, V, top = (1 << 20) + 1537, 27, 2
+    block, some, gen = make(1024, V, dt, 47)
+    a, h, c = ups(gen, (1024,), top)
+    out = check(block, some, top, up=(a, h, c))
+    again = lambda t: t.repeat(1026, *[1] * (t.dim() - 1))[:rows]  # noqa: E731
+    x = again(block).requires_grad_(True)
+    many = kernel.token_logprobs(x, again(some), top)
+    assert all(torch.equal(m, again(o)) for m, o in zip(many, out))
+    for upstream in ((a,), (a, h, c)):   # a vector a thread, and two
+        y = block.requires_grad_(True)
+        want, = torch.autograd.grad(kernel.token_logprobs(y, some, top)[:len(upstream)], y, upstream)
+        got, = torch.autograd.grad(many[:len(upstream)], x, [again(u) for u in upstream], retain_graph=True)
+        assert torch.equal(got, again(want))
+
+
 def test_offsets_past_32_bits():
     say("token_logprobs rows past 2^32 bytes and 2^31 elements")
     rows, V = 70000, 32000

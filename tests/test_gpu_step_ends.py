@@ -29,8 +29,9 @@ def _batch(B, T, V, seed, ignored=0.1):
 @pytest.mark.parametrize("autocast", [False, True])
 def test_loss_is_the_forwards(autocast):
     """UnifiedLM.loss against the float64 cross-entropy of forward's logits, and its gradients against
-    those of their cross-entropy in fp32 (under autocast F.cross_entropy itself is coarser). The logits' gradients then differ by roundings of fp32 sums, which tip one in some thousand
-    of the bf16 roundings that follow, 2^-8 of its value each."""
+    those of their cross-entropy in fp32 (under autocast F.cross_entropy itself is coarser). The logits'
+    gradients then differ by roundings of fp32 sums, which tip one in some thousand of the bf16 roundings
+    that follow, 2^-8 of its value each."""
     say(f"loss against forward, autocast={autocast}")
     model = _model(dim=64, hidden_dim=96)
     x, y = _batch(3, 37, 97, 1)

@@ -137,11 +137,14 @@ def test_the_entries_refuse_before_any_hip_call():
         assert lib.ulm_embed_fwd(*a) == nat.ULM_ERR_INVALID and msg in lib.ulm_last_error()
     need = lib.ulm_embed_bwd_workspace_bytes(4, 10, 8)
     assert need > 0 and lib.ulm_embed_bwd_workspace_bytes(0, 10, 8) == 0
-    for a, msg in (((X, 0, X, 4, 10, 8, 1.0, X, X, need - 1, None), b"workspace"), ((X, 0, X, 4, 10, 8, 1.0, None, X, need, None), b"null")):
+    for a, msg in (((X, 0, X, 4, 10, 8, 1.0, X, X, need - 1, None), b"workspace"),
+                   ((X, 0, X, 4, 10, 8, 1.0, None, X, need, None), b"null")):
         assert lib.ulm_embed_bwd(*a) == nat.ULM_ERR_INVALID and msg in lib.ulm_last_error()
-    grad = lambda **kw: (nat.Grad * 1)(nat.Grad(**{**dict(src=256, dst=512, numel=5, src_dtype=0, dst_dtype=0), **kw}))  # noqa: E731
+    grad = lambda **kw: (nat.Grad * 1)(  # noqa: E731
+        nat.Grad(**{**dict(src=256, dst=512, numel=5, src_dtype=0, dst_dtype=0), **kw}))
     clip = lambda g, n=1, kind=2, bound=1.0, ws=1 << 20: lib.ulm_clip_grads(g, n, kind, bound, X, X, ws, None)  # noqa: E731
-    for g, kw, msg in ((grad(numel=-1), {}, b"elements"), (grad(src_dtype=5), {}, b"bad dtype"), (grad(dst_dtype=5), {}, b"bad dtype"),
+    for g, kw, msg in ((grad(numel=-1), {}, b"elements"), (grad(src_dtype=5), {}, b"bad dtype"),
+                       (grad(dst_dtype=5), {}, b"bad dtype"),
                        (grad(src=None), {}, b"null pointer"), (grad(dst=None), {}, b"null pointer"), (None, {}, b"null pointer"),
                        (grad(dst=256, dst_dtype=1), {}, b"in place"), (grad(), dict(kind=1), b"norm type"),
                        (grad(), dict(bound=-1.0), b"negative"), (grad(), dict(bound=math.nan), b"negative"),
