@@ -23,7 +23,7 @@ constexpr int kMaxTopV = 1 << 22;      // columns with alternatives: kMaxParts p
 constexpr float kLog2e = 1.44269504088896341f;
 constexpr float kLn2 = 0.693147180559945309f;
 constexpr float kFloor = -1e4f;       // 2^t and e^d are 0 from here on: keeps 0 x (-inf) out of the sums
-constexpr float kHuge = 0x1p96f;      // maxima beyond which m log2(e) is not formed
+constexpr float kHuge = 0x1p24f;      // maxima from which on m log2(e) is not formed: its rounding is at most 1 below
 
 typedef uint32_t u32x4_any __attribute__((vector_size(16), aligned(2)));   // rows may start anywhere
 
@@ -119,23 +119,26 @@ template <int W> __device__ __forceinline__ Sums group_add(Sums v) {
 // A thread's running sums in powers of two about ref = m log2(e), rounded: s = sum 2^t_i,
 // u = sum 2^t_i t_i with t_i = x_i log2(e) - ref in one fused operation (5.5 instructions an
 // element, conversion and maximum included, where differences from m itself and a guard for
-// masked ones take 8: at 16384 rows of 32000 bf16 the ALUs were busy 83% of 204 us). What ref
-// lacks of m log2(e) is put right at the end. Where |m| is so large that ref could
-// overflow (rows masked with the type's lowest value), t_i = (x_i - m) log2(e).
+// masked ones take 8: at 16384 rows of 32000 bf16 the ALUs were busy 83% of 204 us). The largest t is
+// what ref lacks of m log2(e), half a step of ref: at most 1 below kHuge, and put right at the
+// end. From kHuge on (rows masked with a large negative number, say) the powers
+// 2^t would leave fp32's range: there t_i = (x_i - m) log2(e).
 struct Running {
     float m = -INFINITY, s = 0.f, u = 0.f;
     static __device__ __forceinline__ float ref(float m) { return m * kLog2e; }
-    __device__ __forceinline__ bool plain() const { return fabsf(m) < kHuge; }
+    static __device__ __forceinline__ bool plain(float m) { return fabsf(m) < kHuge; }
+    static __device__ __forceinline__ float lacks(float m) { return plain(m) ? __builtin_fmaf(m, kLog2e, -ref(m)) : 0.f; }
+    __device__ __forceinline__ bool plain() const { return plain(m); }
     __device__ __forceinline__ void rebase(float to) {   // to > m
-        const float d = plain() && fabsf(to) < kHuge ? ref(m) - ref(to) : (m - to) * kLog2e;
+        const float d = plain() && plain(to) ? ref(m) - ref(to) : __builtin_fmaf(m - to, kLog2e, lacks(to) - lacks(m));
         const float t = fmaxf(d, kFloor), f = __builtin_amdgcn_exp2f(t);   // m = -inf: s and u are 0
         u = f * __builtin_fmaf(s, t, u);
         s *= f;
         m = to;
     }
     __device__ __forceinline__ Sums sums() const {
-        const float lacks = plain() ? __builtin_fmaf(m, kLog2e, -ref(m)) : 0.f, f = __builtin_amdgcn_exp2f(-lacks);
-        return {m, s * f, kLn2 * f * __builtin_fmaf(-lacks, s, u)};
+        const float l = lacks(m), f = __builtin_amdgcn_exp2f(-l);
+        return {m, s * f, kLn2 * f * __builtin_fmaf(-l, s, u)};
     }
 };
 
