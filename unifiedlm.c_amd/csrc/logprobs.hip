@@ -130,7 +130,9 @@ struct Running {
     static __device__ __forceinline__ float lacks(float m) { return plain(m) ? __builtin_fmaf(m, kLog2e, -ref(m)) : 0.f; }
     __device__ __forceinline__ bool plain() const { return plain(m); }
     __device__ __forceinline__ void rebase(float to) {   // to > m
-        const float d = plain() && plain(to) ? ref(m) - ref(to) : __builtin_fmaf(m - to, kLog2e, lacks(to) - lacks(m));
+        // not ref(m) - ref(to): fused into one operation it takes m log2(e) for ref(m), unrounded, and the sums of a
+        // row about 6e4 come out off by 1e-4
+        const float d = __builtin_fmaf(m - to, kLog2e, lacks(to) - lacks(m));
         const float t = fmaxf(d, kFloor), f = __builtin_amdgcn_exp2f(t);   // m = -inf: s and u are 0
         u = f * __builtin_fmaf(s, t, u);
         s *= f;
