@@ -346,10 +346,20 @@ class UnifiedLM(nn.Module):
         self.last_loss = F.cross_entropy(logits.flatten(0, 1), targets.flatten(), ignore_index=-1)
         return logits
 
+    def _embed(self, tokens):
+        """self.tok_embeddings(tokens) by kernel.embedding (its gradient summed in a fixed order), unless the
+        module is another one, is hooked or does more than look rows up."""
+        emb = self.tok_embeddings
+        if (type(emb) is nn.Embedding and "forward" not in emb.__dict__
+                and emb.padding_idx is None and emb.max_norm is None and not emb.sparse and not emb.scale_grad_by_freq
+                and not (emb._forward_hooks or emb._forward_pre_hooks or emb._backward_hooks or emb._backward_pre_hooks
+                         or _any_global_hook())):
+            return embedding(emb.weight, tokens)
+        return emb(tokens)
+
     def _hidden(self, tokens):
-        """What the classifier reads (B, T, dim), the embedding's rows gathered (and its gradient
-        summed in a fixed order) by kernel.embedding."""
-        h = self.dropout(embedding(self.tok_embeddings.weight, tokens))
+        """What the classifier reads (B, T, dim), the embedding's rows by _embed."""
+        h = self.dropout(self._embed(tokens))
         for layer in self.layers:
             h = layer(h)
         return self.norm(h)
