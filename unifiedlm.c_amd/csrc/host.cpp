@@ -588,6 +588,13 @@ void check_capture(const Tensor &leaf) {
                 "that graph's outputs first");
 }
 
+// the same for calls that the registered ops serve
+void check_capture_of(const py::handle &h) {
+    if (!THPVariable_Check(h.ptr())) return;
+    const Tensor &t = THPVariable_Unpack(h.ptr());
+    if (t.defined() && t.is_cuda()) check_capture(t);
+}
+
 struct TokenLogprobs : torch::autograd::Function<TokenLogprobs> {
     // (logprob, entropy, top_logprobs, top_tokens); the statistics too where `stats` is given
     static variable_list compute(const Tensor &logits, const Tensor &tok, int64_t top, int64_t ignore, Tensor *stats) {
@@ -892,6 +899,7 @@ PYBIND11_MODULE(ulm_host, m) {
     m.def("prefill", &prefill);
     m.def("copies", &copies);
     m.def("decode_step", &decode_step);
+    m.def("check_capture", &check_capture_of);
     m.def("token_logprobs", &token_logprobs);
     m.def("embedding", &embedding);
     m.def("grad_norm", &grad_norm);

@@ -902,6 +902,12 @@ def _token_logprobs_backward(ctx, dlogprob, dentropy, dtop, _dtokens, _dstats):
 torch.library.register_autograd("ulm::token_logprobs", _token_logprobs_backward, setup_context=_token_logprobs_setup)
 
 
+def _check_capture(leaf):
+    """What the host module refuses of a call that is being captured, for the calls it does not take."""
+    if not torch.compiler.is_compiling() and torch.cuda.is_initialized() and torch.cuda.is_current_stream_capturing():
+        nat.host().check_capture(leaf)
+
+
 def _check_tokens(tokens):
     if not isinstance(tokens, torch.Tensor):
         raise TypeError("tokens must be a tensor")
@@ -944,6 +950,7 @@ def token_logprobs(logits, tokens, top=0, ignore_index=-1):
         raise ValueError(f"at most 2^30 columns, 2^22 with alternatives, got {V}")
     nat.dtype_code(logits.dtype)
     nat.require_device(logits, tokens)
+    _check_capture(logits)
     return TokenLogprobs(*token_logprobs_fwd(logits, tokens, top, ignore_index)[:4])
 
 
@@ -1028,6 +1035,7 @@ def embedding(weight, tokens, scale=1.0):
         raise ValueError(f"weight at most 2^28 x 2^20 and 2^30 tokens, got {tuple(weight.shape)} and {tokens.numel()}")
     nat.dtype_code(weight.dtype)
     nat.require_device(weight, tokens)
+    _check_capture(weight)
     return embed_fwd(weight, tokens, float(scale))
 
 
