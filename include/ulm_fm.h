@@ -402,8 +402,9 @@ int ulm_decode_step(const ulm_decode_layer *layers, int n_layers, const float *x
  *                            NULL: not wanted
  * A row of -inf only has logprob and top_logprobs -inf (0 if ignored), entropy 0, top_tokens
  * 0, 1, .. and gradient 0. A row with a NaN or +inf has NaN throughout (but for top_tokens and
- * an ignored token's 0). Workspace of ulm_token_logprobs_workspace_bytes() bytes (may be 0: few
- * rows are split over several workgroups each and joined in a second launch).
+ * an ignored token's 0). Workspace of ulm_token_logprobs_workspace_bytes() bytes: 0, unless top > 0
+ * and the rows are wider than one workgroup's table holds (65536 columns of fp32, 131072 of 16 bits):
+ * those are cut into parts, which a second launch joins.
  *
  * ulm_token_logprobs_bwd: dlogits (rows, V) dense, in dtype, not aliasing logits, from the same
  * arguments, the outputs stats, entropy (with dentropy) and top_tokens (with dtop) and the

@@ -382,22 +382,23 @@ template <int N> __device__ __forceinline__ float take(const float (&x)[N], bool
     return most;
 }
 
-// One workgroup of NT threads per (row, part). With one part it writes the row's outputs, with
-// more the part's sums and its `top` best keys in order (0 where it has fewer). One pass over the
+// One workgroup of NT threads per (row, part). With one part, as always without alternatives, it writes the
+// row's outputs, with more the part's sums and its `top` best keys in order (0 where it has fewer). One pass over the
 // row, which bounds it: 16384 rows of 32000 bf16 157 us, 6.7 TB/s. Workgroups that go from row to row with the
 // next loads ahead took 197 (118 registers leave half the waves), the alternatives 30 more.
 template <int DT, bool TOP, int NT>
 __global__ __launch_bounds__(NT) void fwd_kernel(Rows a, Outs o, Sums *part_sums, uint64_t *part_keys) {
     using T = Tile<DT, NT>;
     constexpr int V = T::vec, W = NT / kWave;
-    const long long id = block_id(), r = a.parts == 1 ? id : id / a.parts;
+    const int parts = TOP ? a.parts : 1;
+    const long long id = block_id(), r = parts == 1 ? id : id / parts;
     if (r >= a.rows) return;
-    const int tid = threadIdx.x, part = static_cast<int>(id - r * a.parts);
+    const int tid = threadIdx.x, part = static_cast<int>(id - r * parts);
     const char *row = a.row(r, Elem<DT>::bytes);
-    const int e0 = part * a.part_len, e1 = min(a.V, e0 + a.part_len);
+    const int e0 = TOP ? part * a.part_len : 0, e1 = TOP ? min(a.V, e0 + a.part_len) : a.V;
     __shared__ std::conditional_t<TOP, TopScratch<NT>, int> scratch;
 
-    const Target to = a.parts == 1 && tid == 0 ? target_of<DT>(a, row, r) : Target{};
+    const Target to = parts == 1 && tid == 0 ? target_of<DT>(a, row, r) : Target{};
     Running v;
     bool masked = false;   // -inf was met: its t is kept finite from then on
     for (int k = 0; e0 + k * T::size < e1; ++k) {
@@ -436,7 +437,7 @@ __global__ __launch_bounds__(NT) void fwd_kernel(Rows a, Outs o, Sums *part_sums
     if (tid < kWave) {
         const Sums all = group_add<W>(waves[tid % W]);
         if (tid == 0) {
-            if (a.parts == 1) finish_row(a, o, r, to, all, ml[0], ml[1]);
+            if (parts == 1) finish_row(a, o, r, to, all, ml[0], ml[1]);
             else part_sums[id] = all;
         }
     }
@@ -448,40 +449,38 @@ __global__ __launch_bounds__(NT) void fwd_kernel(Rows a, Outs o, Sums *part_sums
             int rank = 0;
             for (int j = 0; j < n; ++j) rank += scratch.list[j] > k;
             if (rank >= a.top) continue;
-            if (a.parts == 1) put_top(a, o, r, rank, k, m, logs);
+            if (parts == 1) put_top(a, o, r, rank, k, m, logs);
             else part_keys[id * a.top + rank] = k;
         }
-        if (a.parts > 1)
+        if (parts > 1)
             for (int i = n + tid; i < a.top; i += NT) part_keys[id * a.top + i] = 0;
     }
 }
 
 constexpr int kThreads = 256;   // of the kernels below
 
-// The parts of a row joined: one workgroup per row.
-template <int DT, bool TOP>
+// The parts of a row with alternatives joined: one workgroup per row.
+template <int DT>
 __global__ __launch_bounds__(kThreads) void join_kernel(Rows a, Outs o, const Sums *part_sums, const uint64_t *part_keys) {
     const long long r = block_id();
     if (r >= a.rows) return;
     const int tid = threadIdx.x;
     __shared__ float ml[2];
-    __shared__ uint64_t list[TOP ? kMaxParts * kMaxTop : 1];
-    const int n = TOP ? a.parts * a.top : 0;
+    __shared__ uint64_t list[kMaxParts * kMaxTop];
+    const int n = a.parts * a.top;
     for (int i = tid; i < n; i += kThreads) list[i] = part_keys[r * n + i];
     if (tid < kWave) {   // at most a wave's lanes of parts
         const Sums all = group_add<kWave>(tid < a.parts ? part_sums[r * a.parts + tid] : Sums{-INFINITY, 0.f, 0.f});
         if (tid == 0) finish_row(a, o, r, target_of<DT>(a, a.row(r, Elem<DT>::bytes), r), all, ml[0], ml[1]);
     }
-    if constexpr (TOP) {
-        __syncthreads();
-        const float m = ml[0], logs = ml[1];
-        for (int i = tid; i < n; i += kThreads) {
-            const uint64_t k = list[i];
-            if (k == 0) continue;
-            int rank = 0;
-            for (int j = 0; j < n; ++j) rank += list[j] > k;
-            if (rank < a.top) put_top(a, o, r, rank, k, m, logs);
-        }
+    __syncthreads();
+    const float m = ml[0], logs = ml[1];
+    for (int i = tid; i < n; i += kThreads) {
+        const uint64_t k = list[i];
+        if (k == 0) continue;
+        int rank = 0;
+        for (int j = 0; j < n; ++j) rank += list[j] > k;
+        if (rank < a.top) put_top(a, o, r, rank, k, m, logs);
     }
 }
 
@@ -644,8 +643,8 @@ extern "C" int ulm_token_logprobs(const void *logits, int dtype, const long long
         else if (plan.threads == 128) lp::fwd_kernel<DT, TOP, 128><<<grid, dim3(128), 0, s>>>(a, o, sums, keys);
         else if (plan.threads == 256) lp::fwd_kernel<DT, TOP, 256><<<grid, dim3(256), 0, s>>>(a, o, sums, keys);
         else lp::fwd_kernel<DT, TOP, 512><<<grid, dim3(512), 0, s>>>(a, o, sums, keys);
-        if (parts > 1)
-            lp::join_kernel<DT, TOP><<<lp::grid_of(rows), dim3(lp::kThreads), 0, s>>>(a, o, sums, keys);
+        if constexpr (TOP)
+            if (parts > 1) lp::join_kernel<DT><<<lp::grid_of(rows), dim3(lp::kThreads), 0, s>>>(a, o, sums, keys);
     };
     auto by_top = [&](auto dt) {
         if (top) launch(dt, std::true_type{});
