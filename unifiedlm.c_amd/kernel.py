@@ -926,8 +926,10 @@ def token_logprobs(logits, tokens, top=0, ignore_index=-1):
       top_tokens   (..., top) and those tokens, the lower first on ties
 
     fp32 from fp32, bf16 or fp16 logits, differentiable in them through the first three (dlogits in the
-    logits' dtype). Masked logits (-inf) have probability 0; a row of nothing else has logprob and
-    top_logprobs -inf, entropy 0 and no gradient. Any view whose last dimension is dense is read in
+    logits' dtype). Masked logits (-inf, or any large negative number) have probability 0; a row of -inf
+    alone has logprob and top_logprobs -inf, entropy 0 and no gradient. Equal calls give equal bits; a row's
+    last bits may differ between calls of up to 512 rows and of more, which share a row among more or fewer
+    threads. Any view whose last dimension is dense is read in
     place (logits[:, :-1], say). The loss of a training step is -logprob summed over the tokens
     that count."""
     if _plain_eager():
@@ -1015,7 +1017,7 @@ torch.library.register_autograd("ulm::embed_fwd", _embed_backward, setup_context
 
 def embedding(weight, tokens, scale=1.0):
     """scale * weight[tokens]: weight (V, D) fp32, bf16 or fp16, tokens (...) integer, the result
-    (..., D) in the weight's dtype, rounded once. A token outside [0, V) gives a row of NaN.
+    (..., D) in the weight's dtype, multiplied in fp32 and rounded from it. A token outside [0, V) gives a row of NaN.
     The weight's gradient is dense, in its dtype: each row the fp32 sum of its tokens' gradients in
     an order that the tokens alone fix, so that equal inputs give equal bits; tokens outside [0, V) add
     nothing."""

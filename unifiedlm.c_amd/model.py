@@ -369,7 +369,8 @@ class UnifiedLM(nn.Module):
         not -1, NaN where there are none) on kernel.embedding and kernel.token_logprobs: the
         logits are read once for the loss and once for their gradient, in the dtype the classifier
         gives them (bf16 under bf16 autocast), without the fp32 copies of a log-softmax. entropy_weight
-        takes that share of the same positions' mean entropy off it. last_loss is set as by `forward`."""
+        takes that share of the same positions' mean entropy off it. last_loss is set as by `forward`, and
+        holds the step's graph until the next one."""
         if targets.shape != tokens.shape:
             raise ValueError(f"targets {tuple(targets.shape)} must have the tokens' shape {tuple(tokens.shape)}")
         out = token_logprobs(self.output(self._hidden(tokens)), targets)
@@ -385,7 +386,7 @@ class UnifiedLM(nn.Module):
         """Log probabilities of given tokens (kernel.token_logprobs): of `targets` (B, T; -1 for those that do
         not count) at the positions of tokens (B, T), or without targets of each token after the first
         under the ones before it, (B, T - 1). With them every position's entropy and its `top` most
-        likely tokens."""
+        likely tokens. The model's mode counts: in training mode dropout applies, as in `forward`."""
         if targets is None:
             tokens, targets = tokens[:, :-1], tokens[:, 1:]
         elif targets.shape != tokens.shape:
