@@ -422,6 +422,68 @@ int ulm_token_logprobs_bwd(const void *logits, int dtype, const long long *token
                            const float *dlogprob, const float *dentropy, const float *dtop, void *dlogits,
                            void *stream);
 
+/* Distillation from a teacher's top logits, with the log probability of the row's own token beside it.
+ * Rows of logits are addressed as ulm_token_logprobs' (rows, inner, outer_stride, row_stride, V, dtype).
+ *   teacher_tokens (rows, K)  the tokens that the teacher lists, in any order, a token listed again adding its entry;
+ *                             -1: no entry, any other value outside [0, V): the row's loss and gradient are NaN
+ *   teacher_logits (rows, K)  of teacher_dtype: logits up to a constant a row, or, with rest, the teacher's log
+ *                             probabilities at this temperature
+ *   tokens (rows,) or NULL    the row's own token; ignore_index: logprob 0 and no gradient, any other value
+ *                             outside [0, V): NaN
+ * With p = softmax(x / temperature) and q = softmax over the entries of (teacher_logits / temperature):
+ *   loss[r] = sum_k q_k (ln q_k - ln p_(token k))
+ * or, with rest, q_k = e^(teacher_logits_k), q_r = max(0, 1 - sum_k q_k) and p_r the mass of the tokens not listed:
+ *   loss[r] = sum_k q_k (ln q_k - ln p_(token k)) + q_r (ln q_r - ln p_r)
+ * with 0 ln 0 = 0; a row without entries has loss 0 and no gradient of it. An entry of -inf weighs nothing (and is listed);
+ * where p is 0 and q is not, the loss is +inf, its gradient that of the formula (none from an empty rest).
+ *   logprob (rows,) or NULL   out: x_t - ln sum_i e^x_i, at temperature 1
+ *   stats (rows, ulm_distill_stats()) or NULL   out: for the backward
+ * A row of -inf only has no gradient; NaN or +inf among the logits make the outputs NaN.
+ * K at most ulm_distill_max_entries(), V at most 2^30 (2^18 with rest), temperature from 1e-6 to 1e6.
+ *
+ * ulm_distill_bwd: dlogits (rows, V) dense, in dtype, not aliasing logits, from the same arguments, stats and the
+ * gradients of loss and logprob, each (rows,) fp32 or NULL. No gradient goes to the teacher's logits. */
+typedef struct ulm_distillation {
+    const void *logits;
+    const long long *teacher_tokens;
+    const void *teacher_logits;
+    const long long *tokens;
+    long long rows, inner, outer_stride, row_stride, ignore_index;
+    int V, K, dtype, teacher_dtype, rest;
+    float temperature;
+} ulm_distillation;
+int ulm_distill_max_entries(void);
+int ulm_distill_stats(void);
+int ulm_distill(const ulm_distillation *d, float *loss, float *logprob, float *stats, void *stream);
+int ulm_distill_bwd(const ulm_distillation *d, const float *stats, const float *dloss, const float *dlogprob,
+                    void *dlogits, void *stream);
+
+/* Draws one token a row from logits (rows addressed as ulm_token_logprobs'), V at most 2^22.
+ * w_i = e^((x_i - max x) / temperature), -inf (masked) entries having no part. By value down, the lower index first on
+ * ties, the entry of rank j is kept if j = 0, or if
+ *   j < top_k,   the mass (sum of w) of the ranks before it is less than top_p times that of the first top_k ranks,
+ *   and w >= min_p.
+ * The token is the first kept one, in the order of the indices, at which the running sum of kept w exceeds u times their
+ * sum. top_k <= 0, top_p >= 1 and min_p <= 0 keep all; temperature 0, top_k 1 and top_p <= 0 keep the first of the largest.
+ *   u (rows,)          random numbers in [0, 1), fp32, or fp64 with u_double
+ *   temperature .. top_k   one for all rows, or a row's own from the arrays that are not NULL
+ *   token (rows,)      out; -1 where nothing can be drawn: no entry above -inf, a NaN or +inf among the entries,
+ *                      a temperature that is negative, infinite or NaN, a NaN among the settings
+ *   logprob (rows,)    out: ln(w_token / sum of kept w), NaN with token -1
+ *   kept (rows,)       out: the number kept, 0 with token -1
+ * Masses are integers of 2^-(62 - ceil(log2 V)) (at most 2^-47) from exponentials in double, so that their sums do not
+ * depend on an order: a row's results are its own and equal calls give equal bits. A token lighter than half of that
+ * unit is not drawn. */
+typedef struct ulm_sampling {
+    double temperature, top_p, min_p;
+    long long top_k;
+    const float *temperatures, *top_ps, *min_ps;
+    const long long *top_ks;
+} ulm_sampling;
+int ulm_sample_tokens(const void *logits, int dtype, long long rows, long long inner, long long outer_stride,
+                      long long row_stride, int V, const void *u, int u_double, const ulm_sampling *how, long long *token,
+                      float *logprob, long long *kept, void *stream);
+
 /* Embedding lookup (nn.Embedding, model.py:117, 150) and its weight's gradient:
  * out[n] = scale W[tokens[n]], W (V,D) and out (N,D) dense in dtype; a token
  * outside [0, V) gives a row of NaN. dweight[v] = scale times the sum of dout[n]

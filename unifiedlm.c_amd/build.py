@@ -23,7 +23,8 @@ HOST_LIB = os.path.join(HERE, "ulm_host.so")
 INCLUDE = os.path.join(os.path.dirname(HERE), "include")
 
 SOURCES = ["status.hip", "elementwise.hip", "decode.hip", "decode_step.hip", "address.hip", "fm_stats.hip", "fm_chunk.hip", "pair.hip",
-           "fm_chunks.hip", "la_kgroup.hip", "fm_ops.hip", "block.hip", "wgrad.hip", "logprobs.hip", "embed.hip", "grads.hip"]
+           "fm_chunks.hip", "la_kgroup.hip", "fm_ops.hip", "block.hip", "wgrad.hip", "logprobs.hip", "embed.hip", "grads.hip",
+           "distill.hip", "sample.hip"]
 PROBE_SOURCES = ["status.hip", "probe.hip"]   # the test-only probe library
 ARCH = "gfx950"
 FLAGS = [f"--offload-arch={ARCH}", "-O3", "-fPIC", "-std=c++17", "-munsafe-fp-atomics",

@@ -24,6 +24,7 @@
 #include <torch/csrc/utils/pybind.h>
 
 #include <algorithm>
+#include <array>
 #include <limits>
 #include <optional>
 #include <string>
@@ -687,6 +688,209 @@ py::object token_logprobs(const py::handle &logits_, const py::handle &tokens_, 
     return py::make_tuple(py::cast(out[0]), py::cast(out[1]), py::cast(out[2]), py::cast(out[3]));
 }
 
+struct Distill : torch::autograd::Function<Distill> {
+    struct How {
+        double temperature;
+        bool rest;
+        int64_t ignore;
+    };
+    // the arguments that both directions share, and what they point to
+    struct Call {
+        LogitRows r;
+        Tensor ids, values, tok;
+        ulm_distillation d{};
+        Call(const Tensor &logits, const Tensor &teacher, const Tensor &values_, const Tensor &tokens, const How &how)
+            : r(logits), ids(ids64(teacher)), values(values_.contiguous()) {
+            if (tokens.defined()) tok = ids64(tokens);
+            d.logits = r.x.data_ptr();
+            d.teacher_tokens = ip(ids);
+            d.teacher_logits = values.data_ptr();
+            d.tokens = tok.defined() ? ip(tok) : nullptr;
+            d.rows = r.rows;
+            d.inner = r.inner;
+            d.outer_stride = r.outer_stride;
+            d.row_stride = r.row_stride;
+            d.ignore_index = how.ignore;
+            d.V = r.V;
+            d.K = static_cast<int>(ids.size(-1));
+            d.dtype = code(logits.scalar_type());
+            d.teacher_dtype = code(values.scalar_type());
+            d.rest = how.rest;
+            d.temperature = static_cast<float>(how.temperature);
+        }
+    };
+    // (loss, logprob where there are tokens); the statistics too where `stats` is given
+    static variable_list compute(const Tensor &logits, const Tensor &teacher, const Tensor &values, const Tensor &tokens,
+                                 const How &how, Tensor *stats) {
+        const c10::DeviceGuard device(logits.device());
+        const Maker make(logits);
+        const auto lead = logits.sizes().slice(0, logits.dim() - 1);
+        const Tensor loss = make(lead), logprob = tokens.defined() ? make(lead) : Tensor();
+        if (stats) {
+            std::vector<int64_t> with(lead.begin(), lead.end());
+            with.push_back(ulm_distill_stats());
+            *stats = make(with);
+        }
+        if (loss.numel()) {
+            const Call c(logits, teacher, values, tokens, how);
+            check("ulm_distill", ulm_distill(&c.d, fpm(loss), logprob.defined() ? fpm(logprob) : nullptr,
+                                             stats ? fpm(*stats) : nullptr, stream_of(logits)));
+        }
+        return {loss, logprob};
+    }
+    static variable_list forward(AutogradContext *ctx, const Tensor &logits, const Tensor &teacher, const Tensor &values,
+                                 const std::optional<Tensor> &tokens, double temperature, bool rest, int64_t ignore) {
+        at::AutoDispatchBelowAutograd guard;
+        Tensor stats;
+        const Tensor tok = tokens.value_or(Tensor());
+        variable_list out = compute(logits, teacher, values, tok, {temperature, rest, ignore}, &stats);
+        ctx->save_for_backward({logits, teacher, values, tok, stats});
+        ctx->saved_data["temperature"] = temperature;
+        ctx->saved_data["rest"] = rest;
+        ctx->saved_data["ignore"] = ignore;
+        ctx->set_materialize_grads(false);
+        if (!tok.defined()) out.pop_back();
+        return out;
+    }
+    static variable_list backward(AutogradContext *ctx, variable_list grads) {
+        variable_list out(7);
+        const auto sv = ctx->get_saved_variables();
+        const Tensor &logits = sv[0], &teacher = sv[1], &values = sv[2], &tokens = sv[3], &stats = sv[4];
+        const How how{ctx->saved_data["temperature"].toDouble(), ctx->saved_data["rest"].toBool(), ctx->saved_data["ignore"].toInt()};
+        grads.resize(2);
+        if (!grads[0].defined() && !grads[1].defined()) return out;
+        if (!launches(grads, sv)) {
+            using T1 = const Tensor &;
+            using O = const std::optional<Tensor> &;
+            using F = Tensor(T1, T1, T1, O, double, bool, c10::SymInt, T1, O, O);
+            auto opt = [](const Tensor &t) { return t.defined() ? std::optional<Tensor>(t) : std::nullopt; };
+            out[0] = registered<F>("ulm::distill_bwd").call(logits, teacher, values, opt(tokens), how.temperature, how.rest,
+                                                            how.ignore, stats, opt(grads[0]), opt(grads[1]));
+            return out;
+        }
+        at::AutoDispatchBelowAutograd guard;
+        const c10::DeviceGuard device(logits.device());
+        out[0] = Maker(logits)(logits.sizes(), logits.scalar_type());
+        if (out[0].numel() == 0) return out;
+        const Call c(logits, teacher, values, tokens, how);
+        const Tensor st = stats.contiguous();
+        Tensor up[2];
+        for (int i = 0; i < 2; ++i)
+            if (grads[i].defined()) up[i] = f32c(grads[i]);
+        check("ulm_distill_bwd", ulm_distill_bwd(&c.d, fp(st), fp(up[0]), fp(up[1]), out[0].data_ptr(), stream_of(logits)));
+        return out;
+    }
+};
+
+// a Python number that is no tensor; false otherwise
+bool number(const py::handle &h, double &v) {
+    if (!PyFloat_CheckExact(h.ptr()) && !PyLong_CheckExact(h.ptr())) return false;
+    v = PyFloat_AsDouble(h.ptr());
+    if (v == -1. && PyErr_Occurred()) {
+        PyErr_Clear();
+        return false;
+    }
+    return true;
+}
+bool integer(const py::handle &h, int64_t &v) {
+    if (!PyLong_CheckExact(h.ptr())) return false;
+    v = PyLong_AsLongLong(h.ptr());
+    if (v == -1 && PyErr_Occurred()) {
+        PyErr_Clear();
+        return false;
+    }
+    return true;
+}
+
+py::object distillation(const py::handle &logits_, const py::handle &teacher_, const py::handle &values_,
+                        const py::handle &tokens_, const py::handle &temperature_, const py::handle &rest_,
+                        const py::handle &ignore_) {
+    Distill::How how{};
+    if (!plain_thread() || !PyBool_Check(rest_.ptr()) || !number(temperature_, how.temperature) || !integer(ignore_, how.ignore))
+        return py::none();
+    how.rest = rest_.ptr() == Py_True;
+    const Tensor logits = plain(logits_), teacher = plain_ids(teacher_), values = plain(values_);
+    const bool labelled = !tokens_.is_none();
+    const Tensor tokens = labelled ? plain_ids(tokens_) : Tensor();
+    if (!logits.defined() || !teacher.defined() || !values.defined() || (labelled && !tokens.defined()) || !has_code(logits) ||
+        !has_code(values) || teacher.device() != logits.device() || values.device() != logits.device() ||
+        (labelled && tokens.device() != logits.device()) || logits.dim() < 1 || teacher.dim() != logits.dim() ||
+        logits.size(-1) == 0 || logits.size(-1) > (how.rest ? 1 << 18 : 1 << 30) || teacher.sizes() != values.sizes() ||
+        !(how.temperature >= 1e-6 && how.temperature <= 1e6))
+        return py::none();
+    const auto lead = logits.sizes().slice(0, logits.dim() - 1);
+    const int64_t K = teacher.size(-1);
+    if (K < 1 || K > ulm_distill_max_entries() || teacher.sizes().slice(0, teacher.dim() - 1) != lead ||
+        (labelled && tokens.sizes() != lead))
+        return py::none();
+    const variable_list out = unlocked([&] {
+        if (wants_grad(logits)) {
+            check_capture(logits);
+            return Distill::apply(logits, teacher, values, labelled ? std::optional<Tensor>(tokens) : std::nullopt,
+                                  how.temperature, how.rest, how.ignore);
+        }
+        at::AutoDispatchBelowAutograd guard;
+        return Distill::compute(logits, teacher, values, tokens, how, nullptr);
+    });
+    return py::make_tuple(py::cast(out[0]), labelled ? py::cast(out[1]) : py::object(py::none()));
+}
+
+// a setting of sample_tokens: a number that `ok` takes, or a plain tensor of the rows' own; false otherwise
+template <class Ok> bool setting(const py::handle &h, const Tensor &logits, double &one, Tensor &each, Ok ok) {
+    if (number(h, one)) return ok(one);
+    each = plain(h);
+    return each.defined() && each.device() == logits.device() && each.sizes() == logits.sizes().slice(0, logits.dim() - 1);
+}
+
+py::object sample_tokens(const py::handle &logits_, const py::handle &u_, const py::handle &temperature, const py::handle &top_k,
+                         const py::handle &top_p, const py::handle &min_p) {
+    if (!plain_thread()) return py::none();
+    const Tensor logits = plain(logits_), u = plain(u_);
+    if (!logits.defined() || !u.defined() || !has_code(logits) || logits.dim() < 1 || logits.size(-1) == 0 ||
+        logits.size(-1) > (1 << 22) || u.device() != logits.device() ||
+        (u.scalar_type() != at::kFloat && u.scalar_type() != at::kDouble) ||
+        u.sizes() != logits.sizes().slice(0, logits.dim() - 1))
+        return py::none();
+    ulm_sampling how{};
+    Tensor Ts, ks, ps, ms;
+    int64_t k = 0;
+    const auto share = [](double v) { return v >= 0 && v <= 1; };
+    if (!setting(temperature, logits, how.temperature, Ts,
+                 [](double v) { return v >= 0 && v < std::numeric_limits<double>::infinity(); }) ||
+        !setting(top_p, logits, how.top_p, ps, share) || !setting(min_p, logits, how.min_p, ms, share))
+        return py::none();
+    if (!integer(top_k, k)) {
+        ks = plain_ids(top_k);
+        if (!ks.defined() || ks.device() != logits.device() || ks.sizes() != u.sizes()) return py::none();
+    } else if (k < 0) {
+        return py::none();
+    }
+    how.top_k = k;
+    const auto out = unlocked([&] {
+        at::NoGradGuard no_grad;
+        at::AutoDispatchBelowAutograd guard;
+        const c10::DeviceGuard device(logits.device());
+        const Maker make(logits);
+        const auto lead = logits.sizes().slice(0, logits.dim() - 1);
+        const Tensor token = make(lead, at::kLong), logprob = make(lead), kept = make(lead, at::kLong);
+        const LogitRows r(logits);
+        if (r.rows) {
+            const Tensor uc = u.contiguous();
+            if (Ts.defined()) how.temperatures = fp(Ts = f32c(Ts));
+            if (ps.defined()) how.top_ps = fp(ps = f32c(ps));
+            if (ms.defined()) how.min_ps = fp(ms = f32c(ms));
+            if (ks.defined()) how.top_ks = ip(ks = ids64(ks));
+            check("ulm_sample_tokens",
+                  ulm_sample_tokens(r.x.data_ptr(), code(logits.scalar_type()), r.rows, r.inner, r.outer_stride, r.row_stride,
+                                    r.V, uc.data_ptr(), u.scalar_type() == at::kDouble, &how,
+                                    static_cast<long long *>(token.data_ptr()), fpm(logprob),
+                                    static_cast<long long *>(kept.data_ptr()), stream_of(logits)));
+        }
+        return std::array<Tensor, 3>{token, logprob, kept};
+    });
+    return py::make_tuple(py::cast(out[0]), py::cast(out[1]), py::cast(out[2]));
+}
+
 struct Embedding : torch::autograd::Function<Embedding> {
     static Tensor compute(const Tensor &weight, const Tensor &tokens, double scale) {
         const c10::DeviceGuard device(weight.device());
@@ -901,6 +1105,8 @@ PYBIND11_MODULE(ulm_host, m) {
     m.def("decode_step", &decode_step);
     m.def("check_capture", &check_capture_of);
     m.def("token_logprobs", &token_logprobs);
+    m.def("distillation", &distillation);
+    m.def("sample_tokens", &sample_tokens);
     m.def("embedding", &embedding);
     m.def("grad_norm", &grad_norm);
     m.def("clip_grads", &clip_grads);

@@ -17,7 +17,10 @@ Besides the operator this module exposes the relu^2 slot address
 kernels used by UnifiedBlock.step, and the two ends of a step: the embedding
 lookup, the log probabilities of given tokens (the loss), and the gradients'
 norm and clipping.
+Beside the log probabilities stand the loss that a teacher's top logits give
+(distillation) and the drawing of tokens (sample_tokens).
 """
+import ctypes
 import math
 import operator
 from collections import namedtuple
@@ -954,6 +957,249 @@ def token_logprobs(logits, tokens, top=0, ignore_index=-1):
     nat.require_device(logits, tokens)
     _check_capture(logits)
     return TokenLogprobs(*token_logprobs_fwd(logits, tokens, top, ignore_index)[:4])
+
+
+# ---------------------------------------------------------------------------
+# learning from a teacher's top logits, beside the text's own loss
+
+Distillation = namedtuple("Distillation", "loss logprob")
+MAX_ENTRIES = 1024        # ulm_distill_max_entries()
+DISTILL_STATS = 8         # ulm_distill_stats()
+MAX_REST_V = 1 << 18      # columns with the rest
+
+
+def _distillation(logits, teacher_tokens, teacher_logits, tokens, temperature, rest, ignore_index):
+    """ulm_distillation of contiguous teacher entries and tokens, and what it points to."""
+    x, inner, outer_stride, row_stride = _rows(logits)
+    ids, values = _int_tokens(teacher_tokens), teacher_logits.contiguous()
+    tok = None if tokens is None else _int_tokens(tokens)
+    V = logits.shape[-1]
+    d = nat.Distillation(logits=x.data_ptr(), teacher_tokens=ids.data_ptr(), teacher_logits=values.data_ptr(),
+                         tokens=None if tok is None else tok.data_ptr(), rows=logits.numel() // V, inner=inner,
+                         outer_stride=outer_stride, row_stride=row_stride, ignore_index=ignore_index, V=V, K=ids.shape[-1],
+                         dtype=nat.dtype_code(logits.dtype), teacher_dtype=nat.dtype_code(values.dtype), rest=int(rest),
+                         temperature=temperature)
+    return d, (x, ids, values, tok)
+
+
+@torch.library.custom_op("ulm::distill", mutates_args=())
+def distill_fwd(logits: Tensor, teacher_tokens: Tensor, teacher_logits: Tensor, tokens: Optional[Tensor],
+                temperature: float, rest: bool, ignore_index: int) -> tuple[Tensor, Tensor, Tensor]:
+    """(loss, logprob ((0,) without tokens), stats (..., DISTILL_STATS)): ulm_distill."""
+    lead = logits.shape[:-1]
+    f32 = dict(device=logits.device, dtype=torch.float32)
+    loss, stats = torch.empty(lead, **f32), torch.empty(*lead, DISTILL_STATS, **f32)
+    logprob = torch.empty(0 if tokens is None else lead, **f32)
+    if loss.numel():
+        with torch.cuda.device(logits.device):
+            d, held = _distillation(logits, teacher_tokens, teacher_logits, tokens, temperature, rest, ignore_index)
+            call("ulm_distill", ctypes.byref(d), ptr(loss), ptr(None if tokens is None else logprob), ptr(stats),
+                 nat.stream_of(logits))
+            del held
+    return loss, logprob, stats
+
+
+@distill_fwd.register_fake
+def _distill_fake(logits, teacher_tokens, teacher_logits, tokens, temperature, rest, ignore_index):
+    lead = logits.shape[:-1]
+    e = lambda *shape: logits.new_empty(*shape, dtype=torch.float32)  # noqa: E731
+    return e(lead), e((0,) if tokens is None else lead), e((*lead, DISTILL_STATS))
+
+
+@torch.library.custom_op("ulm::distill_bwd", mutates_args=())
+def distill_bwd(logits: Tensor, teacher_tokens: Tensor, teacher_logits: Tensor, tokens: Optional[Tensor],
+                temperature: float, rest: bool, ignore_index: int, stats: Tensor, dloss: Optional[Tensor],
+                dlogprob: Optional[Tensor]) -> Tensor:
+    """The logits' gradient in their dtype, dense: ulm_distill_bwd."""
+    out = torch.empty(logits.shape, device=logits.device, dtype=logits.dtype)
+    if out.numel():
+        with torch.cuda.device(logits.device):
+            d, held = _distillation(logits, teacher_tokens, teacher_logits, tokens, temperature, rest, ignore_index)
+            up = [None if t is None or t.numel() == 0 else t.float().contiguous() for t in (dloss, dlogprob)]
+            call("ulm_distill_bwd", ctypes.byref(d), ptr(stats.contiguous()), *map(ptr, up), ptr(out),
+                 nat.stream_of(logits))
+            del held
+    return out
+
+
+@distill_bwd.register_fake
+def _distill_bwd_fake(logits, teacher_tokens, teacher_logits, tokens, temperature, rest, ignore_index, stats, dloss,
+                      dlogprob):
+    return torch.empty_like(logits, memory_format=torch.contiguous_format)
+
+
+def _distill_setup(ctx, inputs, output):
+    logits, teacher_tokens, teacher_logits, tokens, *ctx.how = inputs
+    ctx.labelled = tokens is not None
+    ctx.save_for_backward(logits, teacher_tokens, teacher_logits, tokens, output[2])
+    ctx.mark_non_differentiable(*output[2 if ctx.labelled else 1:])
+    ctx.set_materialize_grads(False)
+
+
+def _distill_backward(ctx, dloss, dlogprob, _dstats):
+    dlogprob = dlogprob if ctx.labelled else None
+    if dloss is None and dlogprob is None:
+        return (None,) * 7
+    logits, teacher_tokens, teacher_logits, tokens, stats = ctx.saved_tensors
+    dx = distill_bwd(logits, teacher_tokens, teacher_logits, tokens, *ctx.how, stats, dloss, dlogprob)
+    return (dx, *(None,) * 6)
+
+
+torch.library.register_autograd("ulm::distill", _distill_backward, setup_context=_distill_setup)
+
+
+def distillation(logits, teacher_tokens, teacher_logits, tokens=None, temperature=1.0, rest=False, ignore_index=-1):
+    """How far softmax(logits / temperature) is from a teacher's over the tokens that the teacher lists, as
+    Distillation:
+
+      loss    (...)  sum_k q_k (ln q_k - ln p_k), p_k the student's probability of the k-th listed token and q the
+                     teacher's: softmax(teacher_logits / temperature) over the entries, so that logits and log
+                     probabilities serve alike (token_logprobs' top_logprobs, say), or, with `rest`,
+                     exp(teacher_logits), log probabilities at this temperature; then what they leave of 1 and
+                     the student's mass outside the list are one more term
+      logprob (...)  with tokens (...): their log probabilities at temperature 1, as token_logprobs gives them (0 and no
+                     gradient where a token is ignore_index); None without
+
+    logits (..., V) fp32, bf16 or fp16; teacher_tokens (..., K) integer, up to 1024 entries in any order, -1 where there is
+    none (a position without any has loss 0 and no gradient of it); a token listed again adds its entry.
+    teacher_logits (..., K) fp32, bf16 or fp16; no gradient goes to them. A teacher's token that is neither
+    -1 nor in [0, V) gives NaN, as does a NaN or +inf among the logits. fp32 outputs, differentiable in logits
+    (dlogits in their dtype), both gradients in one pass. A masked logit (-inf) on a token that the teacher gives
+    weight makes the loss +inf. Any view of the logits whose last dimension is dense is read in place. Equal
+    calls give equal bits. The softened loss of a temperature T is usually weighted by T^2 (UnifiedLM.distill does)."""
+    if _plain_eager():
+        out = nat.host().distillation(logits, teacher_tokens, teacher_logits, tokens, temperature, rest, ignore_index)
+        if out is not None:
+            return Distillation._make(out)
+    for name, t in (("logits", logits), ("teacher_logits", teacher_logits)):
+        if not isinstance(t, torch.Tensor):
+            raise TypeError(f"{name} must be a tensor")
+        _check_float(name, t)
+        nat.dtype_code(t.dtype)
+    _check_tokens(teacher_tokens)
+    if logits.dim() < 1 or logits.shape[-1] == 0:
+        raise ValueError(f"logits must be (..., V), got {tuple(logits.shape)}")
+    lead, V = logits.shape[:-1], logits.shape[-1]
+    if teacher_tokens.dim() != logits.dim() or teacher_tokens.shape[:-1] != lead:
+        raise ValueError(f"teacher_tokens {tuple(teacher_tokens.shape)} must be (..., K) with the logits' leading shape, "
+                         f"{tuple(logits.shape)}")
+    if teacher_logits.shape != teacher_tokens.shape:
+        raise ValueError(f"teacher_logits {tuple(teacher_logits.shape)} must have teacher_tokens' shape, "
+                         f"{tuple(teacher_tokens.shape)}")
+    if not 1 <= teacher_tokens.shape[-1] <= MAX_ENTRIES:
+        raise ValueError(f"between 1 and {MAX_ENTRIES} entries a position, got {teacher_tokens.shape[-1]}")
+    if tokens is not None:
+        _check_tokens(tokens)
+        if tokens.shape != lead:
+            raise ValueError(f"tokens {tuple(tokens.shape)} must have the logits' leading shape, {tuple(logits.shape)}")
+    if isinstance(temperature, torch.Tensor):
+        raise TypeError("temperature must be a number")
+    temperature, ignore_index, rest = float(temperature), operator.index(ignore_index), bool(rest)
+    if not 1e-6 <= temperature <= 1e6:
+        raise ValueError(f"temperature must be between 1e-6 and 1e6, got {temperature}")
+    if V > 1 << 30 or (rest and V > MAX_REST_V):
+        raise ValueError(f"at most 2^30 columns, 2^18 with the rest, got {V}")
+    nat.require_device(logits, teacher_tokens, teacher_logits, tokens)
+    _check_capture(logits)
+    loss, logprob, _ = distill_fwd(logits, teacher_tokens, teacher_logits, tokens, temperature, rest, ignore_index)
+    return Distillation(loss, None if tokens is None else logprob)
+
+
+# ---------------------------------------------------------------------------
+# drawing tokens (UnifiedLM.generate, model.py:205-222; sample.py:61)
+
+SampledTokens = namedtuple("SampledTokens", "token logprob kept")
+
+
+@torch.library.custom_op("ulm::sample_tokens", mutates_args=())
+def sample_tokens_op(logits: Tensor, u: Tensor, temperature: float, top_k: int, top_p: float, min_p: float,
+                     temperatures: Optional[Tensor], top_ks: Optional[Tensor], top_ps: Optional[Tensor],
+                     min_ps: Optional[Tensor]) -> tuple[Tensor, Tensor, Tensor]:
+    """(token, logprob, kept): ulm_sample_tokens. The settings of all rows, or a row's own where given."""
+    lead, V = logits.shape[:-1], logits.shape[-1]
+    token = torch.empty(lead, device=logits.device, dtype=torch.int64)
+    logprob, kept = torch.empty_like(token, dtype=torch.float32), torch.empty_like(token)
+    rows = token.numel()
+    if rows:
+        with torch.cuda.device(logits.device):
+            x, inner, outer_stride, row_stride = _rows(logits)
+            uc = u.contiguous()
+            f32 = [None if t is None else t.float().contiguous() for t in (temperatures, top_ps, min_ps)]
+            ks = None if top_ks is None else _int_tokens(top_ks)
+            at = lambda t: None if t is None else t.data_ptr()  # noqa: E731
+            how = nat.Sampling(temperature, top_p, min_p, top_k, *map(at, f32), at(ks))
+            call("ulm_sample_tokens", ptr(x), nat.dtype_code(logits.dtype), rows, inner, outer_stride, row_stride, V,
+                 ptr(uc), int(u.dtype == torch.float64), ctypes.byref(how), ptr(token), ptr(logprob), ptr(kept),
+                 nat.stream_of(logits))
+    return token, logprob, kept
+
+
+@sample_tokens_op.register_fake
+def _sample_tokens_fake(logits, u, temperature, top_k, top_p, min_p, temperatures, top_ks, top_ps, min_ps):
+    e = lambda dtype: logits.new_empty(logits.shape[:-1], dtype=dtype)  # noqa: E731
+    return e(torch.int64), e(torch.float32), e(torch.int64)
+
+
+def _setting(name, v, shape, ok, what):
+    """(number, None) or (0, tensor) of a sampling setting."""
+    if isinstance(v, torch.Tensor):
+        if name == "top_k":
+            _check_tokens(v)
+        else:
+            _check_float(name, v)
+        if v.shape != shape:
+            raise ValueError(f"{name} {tuple(v.shape)} must be a number or have the logits' leading shape, {tuple(shape)}")
+        return 0, v
+    v = operator.index(v) if name == "top_k" else float(v)
+    if not ok(v):
+        raise ValueError(f"{name} must be {what}, got {v}")
+    return v, None
+
+
+@torch.no_grad()
+def sample_tokens(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
+    """One token for every row of logits (..., V), as SampledTokens:
+
+      token   (...) int64  drawn from softmax(logits / temperature) over the kept tokens by the random number u (...) in
+                           [0, 1) (torch.rand's fp32, or fp64): the first kept token, in the order of their numbers, up
+                           to which the kept ones' shares add up to more than u
+      logprob (...) fp32   the log of the share it was drawn with
+      kept    (...) int64  how many tokens were kept
+
+    Kept are, of the tokens by probability (the lower first on ties), the first top_k (0: all), of these the
+    fewest that together hold top_p of their mass, and of these the ones at least min_p times as likely as the
+    first; never none. A masked token (-inf) is never kept. Temperature 0 takes the likeliest token. Each
+    setting is a number or a tensor (...) with a row's own (read as fp32; top_k as integers), and a row's draw depends on
+    that row alone. Where nothing can be drawn (all masked, a NaN or +inf among the logits, a setting in a tensor that is
+    NaN or a temperature there that is negative or infinite) the token is -1, its logprob NaN and kept 0.
+
+    logits fp32, bf16 or fp16, any view whose last dimension is dense read in place, V up to 2^22. Shares are formed and
+    compared to about 1e-12 of a row's mass, in sums that do not depend on an order: equal calls draw equal tokens.
+    No gradient."""
+    if _plain_eager():
+        out = nat.host().sample_tokens(logits, u, temperature, top_k, top_p, min_p)
+        if out is not None:
+            return SampledTokens._make(out)
+    for name, t in (("logits", logits), ("u", u)):
+        if not isinstance(t, torch.Tensor):
+            raise TypeError(f"{name} must be a tensor")
+    _check_float("logits", logits)
+    nat.dtype_code(logits.dtype)
+    if u.dtype not in (torch.float32, torch.float64):
+        raise TypeError(f"u must be float32 or float64, got {u.dtype}")
+    if logits.dim() < 1 or logits.shape[-1] == 0:
+        raise ValueError(f"logits must be (..., V), got {tuple(logits.shape)}")
+    if logits.shape[-1] > 1 << 22:
+        raise ValueError(f"at most 2^22 columns, got {logits.shape[-1]}")
+    lead = logits.shape[:-1]
+    if u.shape != lead:
+        raise ValueError(f"u {tuple(u.shape)} must have the logits' leading shape, {tuple(logits.shape)}")
+    T, Ts = _setting("temperature", temperature, lead, lambda v: 0 <= v < math.inf, "finite and not negative")
+    k, ks = _setting("top_k", top_k, lead, lambda v: 0 <= v < 1 << 63, "not negative")
+    p, ps = _setting("top_p", top_p, lead, lambda v: 0 <= v <= 1, "between 0 and 1")
+    m, ms = _setting("min_p", min_p, lead, lambda v: 0 <= v <= 1, "between 0 and 1")
+    nat.require_device(logits, u, Ts, ks, ps, ms)
+    return SampledTokens(*sample_tokens_op(logits, u, T, k, p, m, Ts, ks, ps, ms))
 
 
 # ---------------------------------------------------------------------------

@@ -18,8 +18,9 @@ weights). Every body here is this package's own:
 The reference's training-loop and sampling helpers keep their signatures
 (configure_optimizers, estimate_mfu, generate: train.py:172, 295, sample.py:61)
 with bodies of this package's own; generate samples on the decode kernels.
-`loss`, `score` and `clip_grad_norm_` run the ends of a training or scoring
-step on the package's kernels as well.
+`loss`, `score`, `distill` and `clip_grad_norm_` run the ends of a training or
+scoring step on the package's kernels as well, `sample` those of a decode
+position.
 """
 import inspect
 import math
@@ -32,8 +33,8 @@ import torch.nn.functional as F
 
 from kernel import (CHUNK, LOG_W_MAX, LOG_W_MIN, TokenLogprobs, block_eager, block_prefill, block_prefill_eager,
                     clip_grad_norm_, decode_addr, decode_addr_deferred, decode_deferred, decode_pre, decode_state,
-                    decode_step, embedding, fm_prefill, matrix_copies, relu2_address, rms_norm, token_logprobs,
-                    unified_block, unified_memory)
+                    decode_step, distillation, embedding, fm_prefill, matrix_copies, relu2_address, rms_norm,
+                    sample_tokens, token_logprobs, unified_block, unified_memory)
 
 # whether any hook is registered for every module (assumed where torch does not say)
 _any_global_hook = getattr(nn.modules.module, "_has_any_global_hook", lambda: True)
@@ -397,6 +398,31 @@ class UnifiedLM(nn.Module):
             logits = self.output(self._hidden(tokens))
         return token_logprobs(logits, targets, top)
 
+    def distill(self, tokens: torch.Tensor, teacher_tokens: torch.Tensor, teacher_logits: torch.Tensor,
+                targets: Optional[torch.Tensor] = None, temperature: float = 1.0, weight: float = 0.5,
+                rest: bool = False) -> torch.Tensor:
+        """The loss of learning from a teacher's top logits (kernel.distillation) at the positions of tokens
+        (B, T): teacher_tokens and teacher_logits (B, T, K), of a teacher's `score(..., top=K)`, say. Without targets
+        temperature^2 times the mean over the positions that have a teacher's entry; with them (B, T; -1 for
+        those that do not count, for the teacher either) `weight` of that and 1 - weight of `loss`'s
+        cross-entropy, from one pass over the logits and one over their gradient. NaN where nothing
+        counts. last_loss is set as by `loss`."""
+        if teacher_tokens.shape[:-1] != tokens.shape:
+            raise ValueError(f"teacher_tokens {tuple(teacher_tokens.shape)} must be (..., K) with the tokens' shape "
+                             f"{tuple(tokens.shape)}")
+        if targets is not None and targets.shape != tokens.shape:
+            raise ValueError(f"targets {tuple(targets.shape)} must have the tokens' shape {tuple(tokens.shape)}")
+        out = distillation(self.output(self._hidden(tokens)), teacher_tokens, teacher_logits, targets, temperature, rest)
+        on = (teacher_tokens != -1).any(-1)
+        if targets is not None:
+            counted = targets != -1
+            on = on & counted
+        loss = temperature ** 2 * torch.where(on, out.loss, 0.0).sum() / on.sum()
+        if targets is not None:
+            loss = weight * loss - (1 - weight) * out.logprob.sum() / counted.sum()
+        self.last_loss = loss
+        return loss
+
     def clip_grad_norm_(self, max_norm: float, norm_type: float = 2.0, error_if_nonfinite: bool = False) -> torch.Tensor:
         """kernel.clip_grad_norm_ of the model's parameters, as the training loop clips before its
         optimizer's step; returns the norm the gradients had."""
@@ -487,6 +513,37 @@ class UnifiedLM(nn.Module):
         return torch.cat(out, 1)
 
     @torch.no_grad()
+    def sample(self, prompt: torch.Tensor, steps: int, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0,
+               u: Optional[torch.Tensor] = None, generator: Optional[torch.Generator] = None, prefill: bool = True):
+        """decode_greedy's loop with every token after the prompt (B, T0) drawn by kernel.sample_tokens, whose settings
+        are numbers or tensors (B,) with a sequence's own (run.c's -t and -p). The random numbers are
+        u (steps + 1 - T0, B), one row a position, or torch.rand's of `generator`. Returns the
+        (B, steps + 1) tokens and the drawn ones' log probabilities (B, steps + 1 - T0) under what they were
+        drawn from."""
+        B, T0 = prompt.shape
+        if steps < T0:
+            raise ValueError(f"steps={steps} is shorter than the prompt ({T0})")
+        n = steps + 1 - T0
+        if u is None:
+            u = torch.rand(n, B, device=prompt.device, generator=generator)
+        elif u.shape != (n, B):
+            raise ValueError(f"u {tuple(u.shape)} must be {(n, B)}")
+        if prefill:
+            logits, states = self.prefill(prompt)
+        else:
+            states = self.init_states(B, prompt.device)
+            for t in range(T0):
+                logits = self.step(prompt[:, t], states)
+        out, logprobs = [prompt], []
+        for i in range(n):
+            nxt = sample_tokens(logits, u[i], temperature, top_k, top_p, min_p)
+            out.append(nxt.token[:, None])
+            logprobs.append(nxt.logprob)
+            if i + 1 < n:
+                logits = self.step(nxt.token, states)
+        return torch.cat(out, 1), torch.stack(logprobs, 1)
+
+    @torch.no_grad()
     def forward_recurrent(self, tokens: torch.Tensor) -> torch.Tensor:
         """Logits (B, T, V) position by position on the decode kernels, with a
         constant-size state per block: what run.c computes (model.py:164-175)."""
@@ -529,7 +586,7 @@ class UnifiedLM(nn.Module):
         return per_token * T * fwdbwd_per_iter / dt / peak_flops
 
     @torch.inference_mode()
-    def generate(self, idx, max_new_tokens, temperature=1.0, top_k=None):
+    def generate(self, idx, max_new_tokens, temperature=1.0, top_k=None, top_p=None, min_p=None):
         """Appends max_new_tokens sampled tokens to idx (B, T0) (model.py:205-222):
         each is drawn from the last position's logits over at most max_seq_len
         preceding tokens, divided by temperature and cut to the top_k largest
@@ -537,13 +594,20 @@ class UnifiedLM(nn.Module):
         sequences are decoded recurrently (one chunked prefill, then one
         decode step per token), which gives the logits of a full forward over
         the same context; once it slides, each token re-reads the window of
-        the last max_seq_len tokens in one chunked pass."""
+        the last max_seq_len tokens in one chunked pass. With top_p or min_p
+        the tokens are drawn by kernel.sample_tokens from torch.rand's numbers
+        (its top_k keeps the lower of equal logits, not all of them)."""
         window = self.params.max_seq_len
         states = None
         for _ in range(max_new_tokens):
             if states is None or idx.size(1) > window:
                 logits, states = self.prefill(idx[:, -window:])
-            nxt = self._sample(logits.float(), temperature, top_k)
+            if top_p is None and min_p is None:
+                nxt = self._sample(logits.float(), temperature, top_k)
+            else:
+                u = torch.rand(logits.shape[0], device=logits.device)
+                nxt = sample_tokens(logits, u, temperature, top_k or 0, 1.0 if top_p is None else top_p,
+                                    min_p or 0.0).token[:, None]
             idx = torch.cat((idx, nxt), dim=1)
             if idx.size(1) <= window:
                 logits = self.step(nxt[:, 0], states)

@@ -16,12 +16,26 @@ ULM_OK, ULM_ERR_INVALID, ULM_ERR_UNSUPPORTED, ULM_ERR_LAUNCH = 0, 1, 2, 3
 ULM_F32, ULM_BF16, ULM_F16 = 0, 1, 2
 DTYPE_CODE = {torch.float32: ULM_F32, torch.bfloat16: ULM_BF16, torch.float16: ULM_F16}
 
-P, I, SZ, F, L = ctypes.c_void_p, ctypes.c_int, ctypes.c_size_t, ctypes.c_float, ctypes.c_longlong
+P, I, SZ, F, L, D = (ctypes.c_void_p, ctypes.c_int, ctypes.c_size_t, ctypes.c_float, ctypes.c_longlong,
+                     ctypes.c_double)
 
 
 class Grad(ctypes.Structure):
     """ulm_grad: one tensor of ulm_grad_norm / ulm_clip_grads."""
     _fields_ = [("src", P), ("dst", P), ("numel", L), ("src_dtype", I), ("dst_dtype", I)]
+
+
+class Distillation(ctypes.Structure):
+    """ulm_distillation: the arguments that ulm_distill and ulm_distill_bwd share."""
+    _fields_ = [("logits", P), ("teacher_tokens", P), ("teacher_logits", P), ("tokens", P), ("rows", L), ("inner", L),
+                ("outer_stride", L), ("row_stride", L), ("ignore_index", L), ("V", I), ("K", I), ("dtype", I),
+                ("teacher_dtype", I), ("rest", I), ("temperature", F)]
+
+
+class Sampling(ctypes.Structure):
+    """ulm_sampling: the settings of ulm_sample_tokens, one for all rows or a row's own."""
+    _fields_ = [("temperature", D), ("top_p", D), ("min_p", D), ("top_k", L), ("temperatures", P), ("top_ps", P),
+                ("min_ps", P), ("top_ks", P)]
 
 
 NORM_TYPES = {2.0: 2, float("inf"): 0}   # ULM_NORM_*
@@ -74,6 +88,11 @@ SIGNATURES = {
     "ulm_token_logprobs_workspace_bytes": (SZ, [L, I, I, I]),
     "ulm_token_logprobs": (I, [P, I, P, L, L, L, L, I, I, L, P, P, P, P, P, P, SZ, P]),
     "ulm_token_logprobs_bwd": (I, [P, I, P, L, L, L, L, I, I, L, P, P, P, P, P, P, P, P]),
+    "ulm_distill_max_entries": (I, []),
+    "ulm_distill_stats": (I, []),
+    "ulm_distill": (I, [P, P, P, P, P]),
+    "ulm_distill_bwd": (I, [P, P, P, P, P, P]),
+    "ulm_sample_tokens": (I, [P, I, L, L, L, L, I, P, I, P, P, P, P, P]),
     "ulm_embed_fwd": (I, [P, I, P, L, I, I, F, P, P]),
     "ulm_embed_bwd_workspace_bytes": (SZ, [L, I, I]),
     "ulm_embed_bwd": (I, [P, I, P, L, I, I, F, P, P, SZ, P]),
