@@ -24,7 +24,7 @@ INCLUDE = os.path.join(os.path.dirname(HERE), "include")
 
 SOURCES = ["status.hip", "elementwise.hip", "decode.hip", "decode_step.hip", "address.hip", "fm_stats.hip", "fm_chunk.hip", "pair.hip",
            "fm_chunks.hip", "la_kgroup.hip", "fm_ops.hip", "block.hip", "wgrad.hip", "logprobs.hip", "embed.hip", "grads.hip",
-           "distill.hip", "sample.hip"]
+           "distill.hip", "sample.hip", "sample_f32.hip", "sample_bf16.hip", "sample_f16.hip"]
 PROBE_SOURCES = ["status.hip", "probe.hip"]   # the test-only probe library
 ARCH = "gfx950"
 FLAGS = [f"--offload-arch={ARCH}", "-O3", "-fPIC", "-std=c++17", "-munsafe-fp-atomics",
