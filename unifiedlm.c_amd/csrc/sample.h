@@ -551,12 +551,13 @@ __device__ __forceinline__ u64 last_key_by_estimate(const Row<DT, NT> &row, cons
     double goal = -1.;
     const int bin = border_bin(above, goal, d.p, sc);
     if (d.mp > 0.) {   // uniform
-        // what min_p keeps lies above this bin; each of the sums is off by a unit an entry and 2^-21 of itself at most
+        // what min_p keeps lies above this bin; each of the sums is off by a unit an entry and, an exponent being rounded to
+        // 2^-19 and the distances to 2^-24 of themselves, 2^-17 of itself at most
         const int after = static_cast<int>(fmin(-log(d.mp) * kBinsPerNat, kBins - 1.)) + 2;
         u64 own = 0;
         for (int i = tid; i < min(after, kBins); i += NT) own += sc.mass[i];
         const u64 most = group_sum(own, sc);
-        idle = after <= bin && static_cast<double>(most) * (1. + 0x1p-9) + 2. * row.n < goal * (1. - 0x1p-9);
+        idle = after <= bin && static_cast<double>(most) * (1. + 0x1p-15) + 2. * row.n < goal * (1. - 0x1p-15);
     }
     if (idle || bin == kBins - 1) {   // uniform
         __syncthreads();
