@@ -161,6 +161,20 @@ def test_sample_loops():
     assert model.generate(prompt, 60, temperature=0.8, top_k=5, top_p=0.9, min_p=0.01).shape == (3, 66)   # past the window
 
 
+def test_sequences_that_cannot_go_on():
+    """Logits that are no numbers: tokens -1 with log probability NaN, and no lookup of row -1."""
+    say("UnifiedLM.sample of logits with NaN")
+    model = tiny_model(14).cuda()
+    prompt, _ = _batch(2, 5, 96, 15)
+    with torch.no_grad():
+        model.output.weight[96, 3] = math.nan
+    toks, lp = model.sample(prompt, 12, top_k=5)
+    assert (toks[:, 5:] == -1).all() and lp.isnan().all() and torch.equal(toks[:, :5], prompt)
+    out = model.generate(prompt, 4, top_p=0.9)
+    assert (out[:, 5:] == 0).all()
+    torch.cuda.synchronize()
+
+
 def _inputs(seed, rows=200, V=3001, K=20):
     gen = torch.Generator(device="cuda").manual_seed(seed)
     f = lambda *s: torch.randn(*s, device="cuda", generator=gen)  # noqa: E731

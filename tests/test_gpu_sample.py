@@ -95,6 +95,29 @@ def test_draws(rows, V, dt):
         check(x, u, **how)
 
 
+MORE = [dict(top_k=65), dict(top_k=128, top_p=0.9), dict(top_k=129), dict(top_k=3000, top_p=0.99), dict(top_p=1 - 1e-9),
+        dict(temperature=8.0, top_p=0.9999), dict(top_p=0.9, min_p=1e-3), dict(top_p=0.3, min_p=1e-3), dict(top_p=0.99, min_p=0.02),
+        dict(temperature=0.05, top_p=0.9), dict(top_k=300, min_p=0.01), dict(temperature=3.0, top_k=128)]
+
+
+@pytest.mark.parametrize("V,dt", [(9000, "fp32"), (9001, "bf16"), (40000, "fp16"), (2001, "fp32"), (150001, "bf16")])
+def test_few_and_many_rows_alike(V, dt):
+    """Every setting over more rows than CUs and over few: equal bits, and the definition's tokens."""
+    say(f"sample_tokens few and many rows V={V} {dt}")
+    n = 270
+    x, u, gen = make(n, V, dt, V + 1, std=2.5)
+    x[5] = x[5].round()
+    x[6, 200:] = -math.inf
+    some = torch.tensor([0, 5, 6, 269], device="cuda")
+    for how in SETTINGS + MORE:
+        out = kernel.sample_tokens(x, u, **how)
+        for i in (0, 135):
+            part = kernel.sample_tokens(x[i:i + 135], u[i:i + 135], **how)
+            assert all(torch.equal(a.nan_to_num(9), b[i:i + 135].nan_to_num(9)) for a, b in zip(part, out)), how
+        want = reference(x[some], u[some], **how)
+        assert torch.equal(out.token[some].cpu(), want[0]) and torch.equal(out.kept[some].cpu(), want[2]), how
+
+
 @pytest.mark.parametrize("V,dt", [(131072, "bf16"), (131073, "fp32"), (200003, "fp16"), (1 << 20, "bf16")])
 def test_large_vocabularies(V, dt):
     say(f"sample_tokens V={V} {dt}")
@@ -176,6 +199,19 @@ def test_equal_logits_and_borders_met_exactly(V):
     x[:, ::2] = -0.0
     x[:, 1::2] = 0.0     # one value
     assert (check(x, u, top_p=0.5, min_p=1.0).kept == V // 2).all()
+
+
+@pytest.mark.parametrize("V,dt", [(32000, "bf16"), (8000, "fp32")])
+def test_large_entries_in_a_few_threads(V, dt):
+    """More entries than the short way holds, all where only a few threads read; a bin with more than the waves hold."""
+    say(f"sample_tokens crowded entries V={V} {dt}")
+    x, u, gen = make(6, V, dt, 18, std=0.5)
+    x[:, 1000:2200] = 9.0
+    x[1, 1000:2200] = torch.linspace(8.9, 9.0, 1200).to(DT[dt]).cuda()
+    x[2, 1000:2200] = torch.linspace(4.0, 30.0, 1200).to(DT[dt]).cuda()
+    for how in (dict(top_k=50), dict(top_k=128), dict(top_k=1100), dict(top_p=0.5), dict(top_k=900, top_p=0.4),
+                dict(top_p=0.97, min_p=0.5)):
+        check(x, u, **how)
 
 
 @pytest.mark.parametrize("dt", ["fp32", "bf16"])

@@ -519,7 +519,8 @@ class UnifiedLM(nn.Module):
         are numbers or tensors (B,) with a sequence's own (run.c's -t and -p). The random numbers are
         u (steps + 1 - T0, B), one row a position, or torch.rand's of `generator`. Returns the
         (B, steps + 1) tokens and the drawn ones' log probabilities (B, steps + 1 - T0) under what they were
-        drawn from."""
+        drawn from. Where nothing can be drawn (a NaN among the logits, say) the token is -1, and the sequence
+        goes on from token 0."""
         B, T0 = prompt.shape
         if steps < T0:
             raise ValueError(f"steps={steps} is shorter than the prompt ({T0})")
@@ -540,7 +541,7 @@ class UnifiedLM(nn.Module):
             out.append(nxt.token[:, None])
             logprobs.append(nxt.logprob)
             if i + 1 < n:
-                logits = self.step(nxt.token, states)
+                logits = self.step(nxt.token.clamp(min=0), states)   # -1 is no row of the embedding
         return torch.cat(out, 1), torch.stack(logprobs, 1)
 
     @torch.no_grad()
@@ -596,7 +597,8 @@ class UnifiedLM(nn.Module):
         the same context; once it slides, each token re-reads the window of
         the last max_seq_len tokens in one chunked pass. With top_p or min_p
         the tokens are drawn by kernel.sample_tokens from torch.rand's numbers
-        (its top_k keeps the lower of equal logits, not all of them)."""
+        (its top_k keeps the lower of equal logits, not all of them; token 0
+        where nothing can be drawn)."""
         window = self.params.max_seq_len
         states = None
         for _ in range(max_new_tokens):
@@ -607,7 +609,7 @@ class UnifiedLM(nn.Module):
             else:
                 u = torch.rand(logits.shape[0], device=logits.device)
                 nxt = sample_tokens(logits, u, temperature, top_k or 0, 1.0 if top_p is None else top_p,
-                                    min_p or 0.0).token[:, None]
+                                    min_p or 0.0).token[:, None].clamp(min=0)
             idx = torch.cat((idx, nxt), dim=1)
             if idx.size(1) <= window:
                 logits = self.step(nxt[:, 0], states)
