@@ -275,7 +275,7 @@ template <int NT> struct Scratch {
     float wave_top[W];
     u64 lo, hi, before, found;
     float low;
-    int held, bin, first, odd, crowded;
+    int held, bin, from, to, first, odd, crowded;
 };
 
 // The sum over the workgroup, on every thread.
@@ -306,8 +306,10 @@ __device__ __forceinline__ void put(const Args &a, long long r, const Draw &d, c
 }
 
 // The bin of sc.mass in which the last kept one lies, and in `above`, what lies above the bins, what lies above it;
-// of all bins' sum comes the goal, where there is none yet (less than 0).
-template <int NT> __device__ __forceinline__ int border_bin(u64 &above, double &goal, double share, Scratch<NT> &sc) {
+// of all bins' sum comes the goal, where there is none yet (less than 0). ABOUT: sc.from .. sc.to are the bins in which
+// it may lie, each of `entries` entries being off by a unit, and all sums by 2^-16 of the whole.
+template <bool ABOUT, int NT>
+__device__ __forceinline__ int border_bin(u64 &above, double &goal, double share, Scratch<NT> &sc, int entries = 0) {
     constexpr int W = NT / kWave, n = kBins / NT;
     const int tid = threadIdx.x, lane = tid % kWave, wave = tid / kWave;
     u64 own[n], sum = 0;
@@ -315,7 +317,10 @@ template <int NT> __device__ __forceinline__ int border_bin(u64 &above, double &
     for (int i = 0; i < n; ++i) sum += own[i] = sc.mass[tid * n + i];
     const u64 to = wave_scan(sum);
     if (lane == kWave - 1) sc.wave_mass[wave] = to;
-    if (tid == 0) sc.bin = kBins - 1;
+    if (tid == 0) {
+        sc.bin = sc.to = kBins - 1;
+        sc.from = 0;
+    }
     __syncthreads();
     u64 before = above + to - sum, all = 0;
 #pragma unroll
@@ -324,12 +329,18 @@ template <int NT> __device__ __forceinline__ int border_bin(u64 &above, double &
         all += sc.wave_mass[i];
     }
     if (goal < 0.) goal = share * static_cast<double>(all);
+    const double off = static_cast<double>(all) * 0x1p-16 + entries;
 #pragma unroll
     for (int i = 0; i < n; ++i) {
-        if (static_cast<double>(before) < goal && !(static_cast<double>(before + own[i]) < goal)) {   // one
+        auto lies_in = [&](double goal) {   // one bin
+            return static_cast<double>(before) < goal && !(static_cast<double>(before + own[i]) < goal);
+        };
+        if (lies_in(goal)) {
             sc.bin = tid * n + i;
             sc.before = before;
         }
+        if (ABOUT && lies_in(goal - off)) sc.from = tid * n + i;
+        if (ABOUT && lies_in(goal + off)) sc.to = tid * n + i;
         before += own[i];
     }
     __syncthreads();
@@ -482,7 +493,7 @@ __device__ __forceinline__ u64 last_key(const Row<DT, NT> &row, const Draw &d, c
         tail = wave_add(tail);
         if (lane == 0 && tail) atomicAdd(&sc.mass[kBins - 1], tail);
         __syncthreads();
-        const int bin = border_bin(above, goal, d.p, sc);
+        const int bin = border_bin<false>(above, goal, d.p, sc);
         if (tid == 0) {
             sc.crowded = 0;
             sc.hi = sc.lo = 0;
@@ -524,9 +535,9 @@ __device__ __forceinline__ u64 last_key(const Row<DT, NT> &row, const Draw &d, c
 // The last key of the top-p set of a whole row, and in sc.wave_mass and sc.wave_count what is kept of each wave's run;
 // 0 where the estimate did not hold.
 //
-// Sums of fp32 exponentials in bins of 1/96 nat say in which bin the last kept one lies. One pass in whole units then
-// adds up what lies above that bin, per wave, and everything, and holds the bin's own entries, among
-// which the border is found. The estimate may be wrong, the bin's entries too many: what the units say is
+// Sums of fp32 exponentials in bins of 1/96 nat say in which bin, or few bins, the last kept one lies. One pass in whole
+// units then adds up what lies above them, per wave, and everything, and holds their entries, among
+// which the border is found. The estimate may be wrong, the entries too many: what the units say is
 // looked at, and nothing is kept of it then. idle: min_p leaves less than top_p would, by more than the estimate may be
 // off.
 template <int DT, int NT>
@@ -549,7 +560,7 @@ __device__ __forceinline__ u64 last_key_by_estimate(const Row<DT, NT> &row, cons
     __syncthreads();
     u64 above = 0;
     double goal = -1.;
-    const int bin = border_bin(above, goal, d.p, sc);
+    const int bin = border_bin<true>(above, goal, d.p, sc, row.n);
     if (d.mp > 0.) {   // uniform
         // what min_p keeps lies above this bin; each of the sums is off by a unit an entry and, an exponent being rounded to
         // 2^-19 and the distances to 2^-24 of themselves, 2^-17 of itself at most
@@ -563,10 +574,10 @@ __device__ __forceinline__ u64 last_key_by_estimate(const Row<DT, NT> &row, cons
         __syncthreads();
         return 0;
     }
-    const double width = d.T / kBinsPerNat;
+    const double width = d.T / kBinsPerNat, from = max(sc.from, bin - 64), to = min(sc.to, bin + 64) + 1;
     const float slack = (fabsf(m) + static_cast<float>(32. * fmin(d.T, 1e30))) * 0x1p-22f;   // of the bins' own roundings
-    const float high = static_cast<float>(mass.m - bin * width) + slack;
-    const float low = fmaxf(static_cast<float>(mass.m - (bin + 1.) * width) - slack, -__FLT_MAX__);
+    const float high = static_cast<float>(mass.m - from * width) + slack;
+    const float low = fmaxf(static_cast<float>(mass.m - to * width) - slack, -__FLT_MAX__);
     Total everything, over;
     int count = 0;   // the wave's
     WaveList<int> vectors{sc.vectors + wave * kRoom, kRoom, 0};   // with an entry of the bin
