@@ -442,7 +442,8 @@ int ulm_token_logprobs_bwd(const void *logits, int dtype, const long long *token
  * K at most ulm_distill_max_entries(), V at most 2^30 (2^18 with rest), temperature from 1e-6 to 1e6.
  *
  * ulm_distill_bwd: dlogits (rows, V) dense, in dtype, not aliasing logits, from the same arguments, stats and the
- * gradients of loss and logprob, each (rows,) fp32 or NULL. No gradient goes to the teacher's logits. */
+ * gradients of loss and logprob, each (rows,) fp32 or NULL (a loss's of 0 takes nothing from the row's entries, not
+ * even NaN). No gradient goes to the teacher's logits. */
 typedef struct ulm_distillation {
     const void *logits;
     const long long *teacher_tokens;

@@ -313,6 +313,39 @@ def test_nan_and_infinity_stay_in_their_rows():
         assert out.loss[2].isnan() and g[2].isnan().all() and out.logprob.isfinite().all() and g[3:].isfinite().all()
 
 
+@pytest.mark.parametrize("T", [1.0, 2.0, 3.0])
+@pytest.mark.parametrize("rest", [False, True])
+def test_padding_takes_nothing_from_its_entries(rest, T):
+    """Positions left out of the loss by torch.where: NaN, infinities and unknown tokens among their entries leave the
+    gradient that clean entries give: the formula's, and the same bits. (With the rest the listed tokens are a sum apart, so
+    that where the list itself is another, rows 3 and 7, the sum of all is rounded in another order: there the formula
+    and its tolerance alone.)"""
+    say(f"distillation padded positions rest={rest} T={T}")
+    x, ids, t, tokens, up = make(9, 5000, 8, "fp32", 30, rest, T)
+    pad = torch.arange(9, device="cuda") % 2 == 1
+    bad_ids, bad_t = ids.clone(), t.clone()
+    bad_t[1, 2], bad_t[3], bad_t[5, 0] = math.nan, math.inf, 1e30
+    bad_ids[7, 4] = 5000
+    bad_ids[3, 1] = bad_ids[3, 0]
+    for labels in (None, tokens):
+        got = []
+        for i, v in ((ids, t), (bad_ids, bad_t)):
+            y = x.clone().requires_grad_(True)
+            out = kernel.distillation(y, i, v, labels, T, rest)
+            total = (torch.where(pad, 0.0, out.loss) * up[0]).sum()
+            if labels is not None:
+                total = total + (out.logprob * up[1]).sum()
+            got += torch.autograd.grad(total, y)
+        want, tol = reference(x, ids, t, labels, T, rest, -1, (torch.where(pad, 0.0, up[0]), None if labels is None else up[1]))
+        for g in got:
+            assert g.isfinite().all()
+            close(g, want[2], U * tol[2] + torch.finfo(x.dtype).eps / 2 * (want[2].abs() + U * tol[2]) + TINY[x.dtype], "dlogits")
+        same = torch.tensor([r for r in range(9) if not rest or r not in (3, 7)], device="cuda")
+        assert torch.equal(got[0][same], got[1][same])
+        if labels is None:
+            assert all((g[pad] == 0).all() for g in got)
+
+
 def _views(V, dt):
     gen = torch.Generator().manual_seed(23)
     f = lambda *s: (torch.randn(*s, generator=gen) * 2).to(DT[dt]).cuda()  # noqa: E731

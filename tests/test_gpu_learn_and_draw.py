@@ -107,6 +107,28 @@ def test_distill_against_its_formula(rest, autocast):
     assert model.distill(x, ids, t, torch.full_like(y, -1)).isnan()
 
 
+def test_distill_of_a_padded_batch():
+    """Targets of -1 leave a position out for the teacher too: what its entries hold changes neither loss nor gradients."""
+    say("distill of a padded batch")
+    model = tiny_model(4, dim=64, hidden_dim=96).cuda()
+    x, y = _batch(3, 29, 97, 5)
+    y = torch.where(torch.arange(29, device="cuda") < torch.tensor([[29], [11], [1]], device="cuda"), y, -1)
+    gen = torch.Generator().manual_seed(6)
+    ids = torch.rand(3, 29, 97, generator=gen).argsort(-1)[..., :7].cuda()
+    t = torch.randn(3, 29, 7, generator=gen).cuda()
+    res = []
+    for fill in (None, math.nan):
+        v, i = t.clone(), ids.clone()
+        if fill is not None:
+            v[y == -1] = fill
+            i[2, 5:] = 97
+        model.zero_grad(set_to_none=True)
+        loss = model.distill(x, i, v, y, temperature=2.0)
+        loss.backward()
+        res.append([loss.detach()] + [p.grad.clone() for p in model.parameters()])
+    assert all(a.isfinite().all() and torch.equal(a, b) for a, b in zip(*res))
+
+
 def test_a_teacher_equal_to_the_student_teaches_nothing():
     """The whole vocabulary listed, the student's own logits: loss 0 and no gradient, to rounding."""
     say("a teacher equal to the student")

@@ -319,9 +319,11 @@ __global__ __launch_bounds__(kThreads) void bwd_kernel(Args a, Grads g, int tile
     __shared__ float value[kMaxEntries];    // and each one's -q / T times the loss's gradient
     __shared__ int twice;
     const float *st = g.stats + r * kStats;
-    const float mu = st[0], lu = st[1], Cu = st[2], Q = st[3], s4 = st[4], s5 = st[5], l1 = st[6];
+    const float mu = st[0], lu = st[1], s4 = st[4], s5 = st[5], l1 = st[6];
     const bool empty = st[7] != 0.f;
     const float A = g.dloss ? g.dloss[r] * a.inv_tau : 0.f;
+    const bool learns = A != 0.f;   // a row that pads takes nothing from its entries, NaN among them neither
+    const float Cu = learns ? st[2] : 0.f, Q = learns ? st[3] : 0.f;
     const bool own = g.dlogprob != nullptr;   // the row's own token has a gradient
     const long long t = own ? a.tokens[r] : a.ignore;
     float da = t != a.ignore ? g.dlogprob[r] : 0.f;
@@ -339,6 +341,7 @@ __global__ __launch_bounds__(kThreads) void bwd_kernel(Args a, Grads g, int tile
         if (REST) return exp2_of(v * kLog2e);
         return s4 == -INFINITY && v == v ? 0.f : exp2_of((v - s4) * a.c - s5);
     };
+    auto part_of = [&](float q) { return learns ? -A * q : 0.f; };
     auto value_at = [&](int k) { return load_as_f32(a.t.values, r * K + k, a.t.dtype); };
     for (int k = tid; k < K; k += kThreads) {
         const long long j = a.t.ids[r * K + k];
@@ -347,7 +350,7 @@ __global__ __launch_bounds__(kThreads) void bwd_kernel(Args a, Grads g, int tile
         const int at = static_cast<int>(j) - e0;
         if (atomicOr(&mask[at / 32], 1u << (at % 32)) >> (at % 32) & 1) twice = 1;
         entry[at] = static_cast<uint16_t>(k);
-        value[k] = -A * q_of(v);
+        value[k] = part_of(q_of(v));
     }
     __syncthreads();
     if (twice) {   // the same token again: its entries' sum, in their order, for each of them
@@ -357,7 +360,7 @@ __global__ __launch_bounds__(kThreads) void bwd_kernel(Args a, Grads g, int tile
             float q = 0.f;
             for (int i = 0; i < K; ++i)
                 if (a.t.ids[r * K + i] == j) q += q_of(value_at(i));
-            value[k] = -A * q;
+            value[k] = part_of(q);
         }
         __syncthreads();
     }

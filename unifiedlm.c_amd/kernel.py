@@ -1063,7 +1063,8 @@ def distillation(logits, teacher_tokens, teacher_logits, tokens=None, temperatur
     logits (..., V) fp32, bf16 or fp16; teacher_tokens (..., K) integer, up to 1024 entries in any order, -1 where there is
     none (a position without any has loss 0 and no gradient of it); a token listed again adds its entry.
     teacher_logits (..., K) fp32, bf16 or fp16; no gradient goes to them. A teacher's token that is neither
-    -1 nor in [0, V) gives NaN, as does a NaN or +inf among the logits. fp32 outputs, differentiable in logits
+    -1 nor in [0, V) gives NaN, as does a NaN or +inf among the logits; a position whose loss has gradient 0 (padding, by
+    torch.where, say) takes nothing from its entries, whatever they hold. fp32 outputs, differentiable in logits
     (dlogits in their dtype), both gradients in one pass. A masked logit (-inf) on a token that the teacher gives
     weight makes the loss +inf. Any view of the logits whose last dimension is dense is read in place. Equal
     calls give equal bits. The softened loss of a temperature T is usually weighted by T^2 (UnifiedLM.distill does)."""
