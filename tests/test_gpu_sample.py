@@ -229,6 +229,22 @@ def test_many_ties_at_the_border(dt):
         check(x, u, **how)
 
 
+@pytest.mark.parametrize("rows,V,dt", [(24, 32000, "bf16"), (260, 6000, "fp16"), (5, 140001, "fp32"), (3, 900, "fp32")])
+def test_top_p_behind_a_large_top_k(rows, V, dt):
+    """top_p's share is of what top_k keeps; ties, masked rows with fewer entries than top_k, and both zeros at top_k's border."""
+    say(f"sample_tokens top_p behind a large top_k rows={rows} V={V} {dt}")
+    x, u, gen = make(rows, V, dt, 21)
+    x[0] = (x[0].float() * 2).round() / 2
+    x[1, 150:] = -math.inf
+    x[2] = -3.0
+    x[2, 5::3], x[2, 1::9] = -0.0, 0.0
+    for k in (129, 200, 1000, 2500):
+        for p, m in ((0.3, 0.0), (0.95, 0.0), (0.9999, 0.0), (0.95, 0.02), (0.9, 1e-4)):
+            check(x, u, top_k=k, top_p=p, min_p=m)
+    check(x, u, top_k=500, top_p=0.9, temperature=0.02)
+    check(x, u, top_k=500, top_p=0.9, temperature=1e4)
+
+
 def test_the_ends_of_the_random_numbers():
     """u = 0 draws the first kept token, numbers next to 1 the last one with a share; outside [0, 1) likewise."""
     say("sample_tokens ends of u")

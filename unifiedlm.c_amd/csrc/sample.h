@@ -153,7 +153,7 @@ __device__ __forceinline__ float wave_max(float x) {
 // The workgroup's row. A wave has `count` tiles of it, 64 vectors each, from element `from` on: its run. Every pass reads
 // the row again, from the caches, but those that look for large entries where LDS holds every vector's largest (table).
 // Held in LDS, one workgroup a CU, a row left the CU idle at its barriers and while it was loaded: 4096 rows of 32000
-// fp32 with top_p took 515 us instead of 364. Held in registers it left the passes too few.
+// fp32 with top_p, 300 us now, took 515 instead of 364 then. Held in registers it left the passes too few.
 template <int DT, int NT> struct Row {
     static constexpr int vec = Elem<DT>::vec, tile = kWave * vec, W = NT / kWave, kBatch = 4;
     const char *row;
@@ -532,23 +532,41 @@ __device__ __forceinline__ u64 last_key(const Row<DT, NT> &row, const Draw &d, c
     return found;
 }
 
-// The last key of the top-p set of a whole row, and in sc.wave_mass and sc.wave_count what is kept of each wave's run;
+// The last key of the top-p set of a row, or of its entries down to key `least` where that is not 0, and in sc.wave_mass and sc.wave_count what is kept of each wave's run;
 // 0 where the estimate did not hold.
 //
 // Sums of fp32 exponentials in bins of 1/96 nat say in which bin, or few bins, the last kept one lies. One pass in whole
 // units then adds up what lies above them, per wave, and everything, and holds their entries, among
 // which the border is found. The estimate may be wrong, the entries too many: what the units say is
 // looked at, and nothing is kept of it then. idle: min_p leaves less than top_p would, by more than the estimate may be
-// off.
+// off. (4096 rows of 32000 bf16 with top_k 1000 and top_p: 529 us, and 703 with an exact search behind top_k.)
 template <int DT, int NT>
 __device__ __forceinline__ u64 last_key_by_estimate(const Row<DT, NT> &row, const Draw &d, const Mass &mass, float m,
-                                                    Scratch<NT> &sc, bool &idle) {
+                                                    u64 least, Scratch<NT> &sc, bool &idle) {
     constexpr int W = NT / kWave, V = Row<DT, NT>::vec, kRoom = kHeld / W;
     const int tid = threadIdx.x, lane = tid % kWave, wave = tid / kWave;
+    const float last = least ? value_of(least) : -INFINITY;
+    const int last_at = index_of(least);
+    // the entries that count of a vector, -inf for the others; false where the wave has none
+    auto counting = [&](const float (&all)[V], int at, float (&x)[V]) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) x[i] = all[i];
+        if (!least) return true;   // uniform
+        bool any = false;
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            const bool in = x[i] > last || (x[i] == last && at + i <= last_at);
+            x[i] = in ? x[i] : -INFINITY;
+            any |= in;
+        }
+        return __any(any) != 0;
+    };
     for (int i = tid; i < kBins; i += NT) sc.mass[i] = 0;
     __syncthreads();
     const float scale = static_cast<float>(fmin(kBinsPerNat * d.inv, 3e38)), c = static_cast<float>(fmin(mass.c, 3e38));
-    row.tiles([&](const float (&x)[V], int) {
+    row.tiles([&](const float (&all)[V], int at) {
+        float x[V];
+        if (!counting(all, at, x)) return;
 #pragma unroll
         for (int i = 0; i < V; ++i) {
             const float away = m - x[i];
@@ -582,7 +600,9 @@ __device__ __forceinline__ u64 last_key_by_estimate(const Row<DT, NT> &row, cons
     int count = 0;   // the wave's
     WaveList<int> vectors{sc.vectors + wave * kRoom, kRoom, 0};   // with an entry of the bin
     __syncthreads();   // the bins' room is for the lists now
-    row.tiles([&](const float (&x)[V], int at) {
+    row.tiles([&](const float (&all)[V], int at) {
+        float x[V];
+        if (!counting(all, at, x)) return;
         everything.begin(mass);
         over.begin(mass);
         bool listed = false;
@@ -602,11 +622,12 @@ __device__ __forceinline__ u64 last_key_by_estimate(const Row<DT, NT> &row, cons
     vectors.settle();
     WaveList<u64> list{sc.list + wave * kRoom, kRoom, 0};
     for (int h = lane; h - lane < min(vectors.count, kRoom); h += kWave) {
-        float x[V];
+        float held[V], x[V];
 #pragma unroll
-        for (int i = 0; i < V; ++i) x[i] = -INFINITY;
+        for (int i = 0; i < V; ++i) held[i] = -INFINITY;
         const int at = h < min(vectors.count, kRoom) ? vectors.at[h] : 0;
-        if (h < min(vectors.count, kRoom)) row.vector(at, x);
+        if (h < min(vectors.count, kRoom)) row.vector(at, held);
+        if (!counting(held, at, x)) continue;
 #pragma unroll
         for (int i = 0; i < V; ++i) list.push(x[i] <= high && x[i] >= low, key_of(x[i], at + i));
     }
@@ -879,7 +900,7 @@ __global__ __launch_bounds__(NT, 4) void sample_kernel(Args a) {
     if (by_k) least = last_key<false>(row, d, mass, m, 0, sc);
     if (by_p) {
         bool idle = false;
-        const u64 found = by_k || d.T > kWide ? 0 : last_key_by_estimate(row, d, mass, m, sc, idle);
+        const u64 found = d.T > kWide ? 0 : last_key_by_estimate(row, d, mass, m, least, sc, idle);
         counted = found && (d.mp <= 0. || mass.real(value_of(found)) >= d.mp);   // min_p takes nothing more away
         if (found) least = found;
         else if (!idle) least = last_key<true>(row, d, mass, m, least, sc);
@@ -987,8 +1008,10 @@ __global__ __launch_bounds__(NT, 4) void sample_kernel(Args a) {
     }
 }
 
-// Threads a row: as many as it has use for; where there are more rows than CUs, no more than two workgroups a CU allow
-// (4096 rows of 32000 fp32 with top_p 345 us with 512, 450 with 1024; 256 rows 57 and 46). The table where it fits.
+// Threads a row: as many as it has use for; where there are more rows than CUs, no more than two workgroups a CU allow.
+// 4096 rows of 32000 fp32 with top_p: 360 us with 256, 348 with 512, 452 with 1024. One row of 8192 fp32 with top_p 13.8
+// with 512 and 16.8 with 1024, without 7.4 and 9.0; of 32000 24.4 and 24.8, 13.5 and 12.7; 64 rows of 128256 bf16 74 and
+// 67, 46 and 37. (Launches one after another.) The table where it fits.
 template <int DT> int launch(Args a, hipStream_t s) {
     constexpr int kTile = Row<DT, 256>::tile;
     const int V = a.v.V;
@@ -1014,7 +1037,7 @@ template <int DT> int launch(Args a, hipStream_t s) {
         return check_launch("ulm_sample_tokens");
     };
     if (V <= 16 * kTile) return run(std::integral_constant<int, 256>{});
-    if (many) return run(std::integral_constant<int, 512>{});
+    if (many || V <= 64 * kTile) return run(std::integral_constant<int, 512>{});
     return run(std::integral_constant<int, 1024>{});
 }
 extern template int launch<ULM_F32>(Args, hipStream_t);
