@@ -346,6 +346,25 @@ def test_padding_takes_nothing_from_its_entries(rest, T):
             assert all((g[pad] == 0).all() for g in got)
 
 
+@pytest.mark.parametrize("dt,rows,V", [("fp32", 2200, 32001), ("bf16", 4200, 32008), ("fp16", 70001, 2003)])
+@pytest.mark.parametrize("T,rest", [(1.0, True), (2.0, False), (1.5, False)])
+def test_more_logits_than_the_cache_holds(dt, rows, V, T, rest):
+    """More than 256 MiB of logits are read otherwise: each row as in a call of few rows, and a few by the formula."""
+    say(f"distillation of many logits {dt} T={T} rest={rest}")
+    assert rows * V * DT[dt].itemsize > 1 << 28
+    x, ids, t, tokens, up = make(300, V, 20, dt, 31, rest, T)
+    few = torch.arange(rows, device="cuda") % 300
+
+    def both(at):
+        y = x[at].requires_grad_(True)
+        out = kernel.distillation(y, ids[at], t[at], tokens[at], T, rest)
+        return out.loss.detach(), out.logprob.detach(), torch.autograd.grad([out.loss, out.logprob], y, [u[at] for u in up])[0]
+    want = both(torch.arange(300, device="cuda"))
+    for got, w in zip(both(few), want):
+        assert all(torch.equal(got[i:i + 300], w[:rows - i]) for i in range(0, rows, 300))
+    check(x[:5], ids[:5], t[:5], tokens[:5], T, rest, up=(up[0][:5], up[1][:5]))
+
+
 def _views(V, dt):
     gen = torch.Generator().manual_seed(23)
     f = lambda *s: (torch.randn(*s, generator=gen) * 2).to(DT[dt]).cuda()  # noqa: E731

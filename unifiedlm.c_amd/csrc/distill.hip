@@ -28,6 +28,7 @@ using namespace rows;
 constexpr int kUnroll = 4;               // 16-byte loads in flight per thread
 constexpr int kMaxEntries = 1024;
 constexpr int kMaxRestV = 1 << 18;       // one bit a column in LDS
+constexpr long long kHeld = 256ll << 20;   // bytes that the last-level cache holds, from the forward to the backward
 constexpr int kStats = 8;                // floats a row kept for the backward
 constexpr float kNaN = __builtin_nanf("");
 
@@ -125,10 +126,14 @@ __device__ __forceinline__ uint32_t bits_at(const uint32_t *mask, int i) {
     return __builtin_amdgcn_alignbit(mask[i / 32 + 1], mask[i / 32], i % 32);
 }
 
+// KEEP, where the cache holds them all: the logits are read as what will be read again. Forward and backward of 2048 rows
+// of 32000 fp32 with the rest 121 us, and 133 with loads that stream in both; of 993 rows of 31999 fp16 46 and 53; of 1 GB
+// of logits 561 and 551.
+//
 // One workgroup of NT threads per row, one pass over it, which bounds it: 8192 rows of 32000 bf16 82 us, 6.4 TB/s; 2048
 // rows of 32000 fp32 with the rest 42 us, 6.2 TB/s. The teacher's entries, the token and their logits are read ahead
 // and end the row on one wave.
-template <int DT, bool REST, Second S, int NT>
+template <int DT, bool REST, Second S, bool KEEP, int NT>
 __global__ __launch_bounds__(NT) void fwd_kernel(Args a, float *loss_out, float *logprob_out, float *stats) {
     constexpr int V = Elem<DT>::vec, B = Elem<DT>::bytes, W = NT / kWave, kTile = NT * V * kUnroll;
     const long long r = block_id();
@@ -168,7 +173,10 @@ __global__ __launch_bounds__(NT) void fwd_kernel(Args a, float *loss_out, float 
         if (n >= V) {   // every load inside the row: the last tile's overhang reads its last elements and drops them
             u32x4_any w[kUnroll];
 #pragma unroll
-            for (int j = 0; j < kUnroll; ++j) w[j] = load_once(row + static_cast<size_t>(min(at(j), n - V)) * B);
+            for (int j = 0; j < kUnroll; ++j) {
+                const char *p = row + static_cast<size_t>(min(at(j), n - V)) * B;
+                w[j] = KEEP ? *reinterpret_cast<const u32x4_any *>(p) : load_once(p);
+            }
 #pragma unroll
             for (int j = 0; j < kUnroll; ++j) unpack<DT>(w[j], *reinterpret_cast<float(*)[V]>(&x[j * V]));
             if (!whole) {
@@ -301,10 +309,10 @@ constexpr int kBwdVectors = 3;   // a thread
 
 // One workgroup per (row, tile of three vectors a thread). The tile's entries are found first, while its elements are
 // under way: a bit and a value a column. Vectors without an entry or the token, nearly all, take
-// their elements alike. Forward and backward of 16384
-// rows of 32000 bf16 with 64 entries 540 us, of 2048 rows fp32 with 32 entries and the rest 129; with one vector a thread
-// 679 and 161, so many workgroups look for their entries, with two 540 and 133, with four 533 and 145.
-template <int DT, bool REST, Second S>
+// their elements alike. Forward and backward of 16384 rows of 32000 bf16 with 64 entries 550 us, of 2048 rows fp32 with
+// 32 entries and the rest 121. (Loads streaming: 540 and 129; with one vector a thread 679 and 161, so many workgroups
+// look for their entries, with two 540 and 133, with four 533 and 145.)
+template <int DT, bool REST, Second S, bool KEEP>
 __global__ __launch_bounds__(kThreads) void bwd_kernel(Args a, Grads g, int tiles) {
     constexpr int V = Elem<DT>::vec, B = Elem<DT>::bytes, U = kBwdVectors, kTile = kThreads * V * U;
     const long long id = a.v.rows * tiles - 1 - block_id();   // from the last row back: the caches hold what was read last
@@ -332,7 +340,7 @@ __global__ __launch_bounds__(kThreads) void bwd_kernel(Args a, Grads g, int tile
 #pragma unroll
     for (int u = 0; u < U; ++u) {
         const int i = e0 + (u * kThreads + tid) * V;
-        if (i < e1) load_vec<DT>(row, i, e1, x[u]);
+        if (i < e1) load_vec<DT, !KEEP>(row, i, e1, x[u]);
     }
     if (tid == 0) twice = 0;
     for (int i = tid; i < kTile / 32 + 1; i += kThreads) mask[i] = 0;
@@ -445,10 +453,15 @@ static ds::Args distill_args(const ulm_distillation *d) {
 template <class F> static void by_kind(const ulm_distillation *d, bool own, F f) {
     using ds::Second;
     const Second second = !own || d->temperature == 1.f ? ds::ONE : d->temperature == 2.f ? ds::SQUARE : ds::TWO;
+    const bool keep = d->rows <= ds::kHeld / d->V / (d->dtype == ULM_F32 ? 4 : 2);
+    auto by_keep = [&](auto dt, auto r, auto s) {
+        if (keep) f(dt, r, s, std::true_type{});
+        else f(dt, r, s, std::false_type{});
+    };
     auto by_second = [&](auto dt, auto r) {
-        if (second == ds::ONE) f(dt, r, std::integral_constant<Second, ds::ONE>{});
-        else if (second == ds::TWO) f(dt, r, std::integral_constant<Second, ds::TWO>{});
-        else f(dt, r, std::integral_constant<Second, ds::SQUARE>{});
+        if (second == ds::ONE) by_keep(dt, r, std::integral_constant<Second, ds::ONE>{});
+        else if (second == ds::TWO) by_keep(dt, r, std::integral_constant<Second, ds::TWO>{});
+        else by_keep(dt, r, std::integral_constant<Second, ds::SQUARE>{});
     };
     auto by_rest = [&](auto dt) {
         if (d->rest) by_second(dt, std::true_type{});
@@ -471,14 +484,15 @@ extern "C" int ulm_distill(const ulm_distillation *d, float *loss, float *logpro
     int nt = 64;
     while (nt < 256 && d->V >= 2 * nt * vec * ds::kUnroll) nt *= 2;
     const size_t lds = d->rest ? (static_cast<size_t>(d->V) / 32 + 2) * 4 : 0;
-    by_kind(d, logprob != nullptr, [&](auto dt, auto rest, auto second) {
+    by_kind(d, logprob != nullptr, [&](auto dt, auto rest, auto second, auto keep) {
         constexpr int DT = decltype(dt)::value;
         constexpr bool R = decltype(rest)::value;
         constexpr ds::Second T = decltype(second)::value;
+        constexpr bool H = decltype(keep)::value;
         const dim3 grid = ds::grid_of(d->rows);
-        if (nt == 64) ds::fwd_kernel<DT, R, T, 64><<<grid, dim3(64), lds, s>>>(a, loss, logprob, stats);
-        else if (nt == 128) ds::fwd_kernel<DT, R, T, 128><<<grid, dim3(128), lds, s>>>(a, loss, logprob, stats);
-        else ds::fwd_kernel<DT, R, T, 256><<<grid, dim3(256), lds, s>>>(a, loss, logprob, stats);
+        if (nt == 64) ds::fwd_kernel<DT, R, T, H, 64><<<grid, dim3(64), lds, s>>>(a, loss, logprob, stats);
+        else if (nt == 128) ds::fwd_kernel<DT, R, T, H, 128><<<grid, dim3(128), lds, s>>>(a, loss, logprob, stats);
+        else ds::fwd_kernel<DT, R, T, H, 256><<<grid, dim3(256), lds, s>>>(a, loss, logprob, stats);
     });
     return check_launch("ulm_distill");
 }
@@ -492,8 +506,8 @@ extern "C" int ulm_distill_bwd(const ulm_distillation *d, const float *stats, co
     const ds::Grads g{stats, dloss, dlogprob, static_cast<char *>(dlogits)};
     hipStream_t s = static_cast<hipStream_t>(stream);
     const int tile = ds::kThreads * ds::kBwdVectors * (d->dtype == ULM_F32 ? 4 : 8), tiles = (d->V + tile - 1) / tile;
-    by_kind(d, dlogprob != nullptr, [&](auto dt, auto rest, auto second) {
-        ds::bwd_kernel<decltype(dt)::value, decltype(rest)::value, decltype(second)::value>
+    by_kind(d, dlogprob != nullptr, [&](auto dt, auto rest, auto second, auto keep) {
+        ds::bwd_kernel<decltype(dt)::value, decltype(rest)::value, decltype(second)::value, decltype(keep)::value>
             <<<ds::grid_of(d->rows * tiles), dim3(ds::kThreads), 0, s>>>(a, g, tiles);
     });
     return check_launch("ulm_distill_bwd");
