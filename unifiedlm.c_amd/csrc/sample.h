@@ -37,8 +37,6 @@ constexpr int kShort = 512;             // and the entries that it ranks
 constexpr int kGroups = 256;            // groups of threads whose maxima bound the k-th largest entry
 constexpr int kTable = 140 << 10, kTableOfTwo = 62 << 10;   // bytes of a row's table in LDS, alone on a CU or with another
 
-constexpr double kWide = 1e36;          // from this temperature on fp32's lowest value may have mass: masked entries are looked for
-
 typedef unsigned long long u64;
 
 struct Setting {
@@ -64,9 +62,14 @@ struct Args {
 // of the sum; that of 2^(52 - bits) rounds w to its units. Its last bit set, w never lies half way
 // between two, so that adding several to one such power rounds each alike, whatever came before: a
 // sum of an entry's w takes 18 instructions.
+//
+// -inf is formed as `floor`, which weighs nothing but where the lowest float lies within some units of t of the maximum:
+// rows of masked entries of that value only, or of such low ones at temperatures past 1e29. There (low) the -inf entries, and what lies past
+// a row's end, are left out by comparison.
 struct Mass {
     double m, c, magic;   // c = log2(e) / T, magic = 2^(52 - bits)
-    float floor;          // entries below have no mass, and t within 32 bits as has this one
+    float floor;          // entries below are formed as this one, whose t is within 32 bits
+    bool low;             // and may have mass
 
     __device__ __forceinline__ Mass(float max, double inv, int bits)
         : m(static_cast<double>(max)), magic(__builtin_ldexp(1., 52 - bits)) {
@@ -76,6 +79,7 @@ struct Mass {
         const uint32_t b = __float_as_uint(max);
         const float below = max > 0.f ? __uint_as_float(b - 1) : max < 0.f ? __uint_as_float(b + 1) : -0x1p-149f;
         floor = fmaxf(fminf(static_cast<float>(m - 0x1p29 / c), below), -__FLT_MAX__);
+        low = (static_cast<double>(floor) - m) * c > -2. - bits;   // half a unit is 2^(-1 - bits)
     }
     __device__ __forceinline__ double real(float x) const {
         constexpr double shift = 6755399441055744.;   // 1.5 2^52
@@ -900,7 +904,7 @@ __global__ __launch_bounds__(NT, 4) void sample_kernel(Args a) {
     if (by_k) least = last_key<false>(row, d, mass, m, 0, sc);
     if (by_p) {
         bool idle = false;
-        const u64 found = d.T > kWide ? 0 : last_key_by_estimate(row, d, mass, m, least, sc, idle);
+        const u64 found = mass.low ? 0 : last_key_by_estimate(row, d, mass, m, least, sc, idle);
         counted = found && (d.mp <= 0. || mass.real(value_of(found)) >= d.mp);   // min_p takes nothing more away
         if (found) least = found;
         else if (!idle) least = last_key<true>(row, d, mass, m, least, sc);
@@ -937,7 +941,7 @@ __global__ __launch_bounds__(NT, 4) void sample_kernel(Args a) {
             row.large_tiles(low, [&](const float (&x)[V], int at) {
                 add(x, [&](float x, int i, double e) { return kept(x, at + i, e); });
             });
-        } else if (by_mp || d.T > kWide) {
+        } else if (by_mp || mass.low) {
             row.large_tiles(low, [&](const float (&x)[V], int) {
                 add(x, [&](float x, int, double e) { return x >= low && e >= d.mp; });
             });
