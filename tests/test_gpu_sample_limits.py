@@ -55,3 +55,15 @@ def test_low_rows_at_temperatures_that_reach_the_lowest_float(dt, T):
     x = _rows(24, 1500, low if dt != torch.float32 else LOWEST * 0.998, low, 5).to(dt).cuda()
     for how in HOW[:10]:
         check(x, _u(24), **{**how, "temperature": T})
+
+
+@pytest.mark.parametrize("T", [5e-324, 1e-310, 5e-309, 1e-300, 1e-200])
+def test_temperatures_whose_reciprocal_is_no_number(T):
+    """The tokens of the largest value share the draw, and its log probability is a number."""
+    say(f"sample_tokens temperature {T}")
+    gen = torch.Generator().manual_seed(3)
+    x = (torch.randn(24, 3000, generator=gen) * 2).cuda()
+    x[::2] = x[::2].round()
+    for how in (dict(), dict(top_k=50), dict(top_k=300), dict(top_p=0.7), dict(top_k=9, top_p=0.5, min_p=0.2), dict(min_p=0.5)):
+        out = check(x, _u(24), temperature=T, **how)
+        assert out.logprob.isfinite().all() and (out.token >= 0).all()

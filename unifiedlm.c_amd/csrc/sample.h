@@ -893,7 +893,7 @@ __global__ __launch_bounds__(NT, 4) void sample_kernel(Args a) {
         return;
     }
 
-    d.T = fmin(d.T, 1e60);   // from there on all are alike
+    d.T = fmin(fmax(d.T, 1e-300), 1e60);   // past these nothing changes any more, and 1 / T is a number
     d.inv = 1. / d.T;
     const Mass mass(m, d.inv, a.bits);
     const bool by_k = k > 1 && k < there, by_p = d.p < 1.;
