@@ -9,6 +9,8 @@ from test_gpu_sample import check
 
 pytestmark = pytest.mark.gpu
 
+import kernel  # noqa: E402
+
 
 def _u(n):
     """Random numbers over all of [0, 1), the last ones next to 1."""
@@ -67,3 +69,20 @@ def test_temperatures_whose_reciprocal_is_no_number(T):
     for how in (dict(), dict(top_k=50), dict(top_k=300), dict(top_p=0.7), dict(top_k=9, top_p=0.5, min_p=0.2), dict(min_p=0.5)):
         out = check(x, _u(24), temperature=T, **how)
         assert out.logprob.isfinite().all() and (out.token >= 0).all()
+
+
+def test_min_p_between_masses_that_rounding_turns_round():
+    """Masses as formed are off by 4e-14, so that an entry a little larger than another may weigh a little less. Whichever of the
+    two a min_p between them keeps, a token comes out of what is kept."""
+    say("sample_tokens min_p between two masses")
+    x = torch.full((64, 5000), -30.0)
+    x[:, 0], x[:, 1], x[:, 2] = 1.0, 0.0, -1e-15
+    T = 2 / math.log(2)   # both weigh 2^-1/2 to 1e-15
+    u = ((torch.arange(64, dtype=torch.float64) + 0.5) / 64).cuda()
+    for k in (0, 200):
+        out = kernel.sample_tokens(x.cuda(), u, T, k, 0.95, 0.707106781186528)
+        assert ((out.kept == 2) | (out.kept == 3)).all(), out.kept
+        assert ((out.token >= 0) & (out.token < 3)).all(), out.token
+        z = 1 + (out.kept.double() - 1) * 2 ** -0.5
+        want = torch.where(out.token == 0, 0.0, -0.5 * math.log(2)) - z.log()
+        assert ((out.logprob - want).abs() <= 2.0 ** -24 * want.abs() + 1e-9).all()

@@ -905,7 +905,8 @@ __global__ __launch_bounds__(NT, 4) void sample_kernel(Args a) {
     if (by_p) {
         bool idle = false;
         const u64 found = mass.low ? 0 : last_key_by_estimate(row, d, mass, m, least, sc, idle);
-        counted = found && (d.mp <= 0. || mass.real(value_of(found)) >= d.mp);   // min_p takes nothing more away
+        // min_p takes nothing more away, nor from larger entries, whose mass as formed may be 4e-14 less
+        counted = found && (d.mp <= 0. || mass.real(value_of(found)) >= d.mp * (1. + 0x1p-40));
         if (found) least = found;
         else if (!idle) least = last_key<true>(row, d, mass, m, least, sc);
     }
