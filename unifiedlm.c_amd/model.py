@@ -405,8 +405,8 @@ class UnifiedLM(nn.Module):
         (B, T): teacher_tokens and teacher_logits (B, T, K), of a teacher's `score(..., top=K)`, say. Without targets
         temperature^2 times the mean over the positions that have a teacher's entry; with them (B, T; -1 for
         those that do not count, for the teacher either) `weight` of that and 1 - weight of `loss`'s
-        cross-entropy, from one pass over the logits and one over their gradient. NaN where nothing
-        counts. last_loss is set as by `loss`."""
+        cross-entropy, from one pass over the logits and one over their gradient; the teacher's part is 0 where no
+        position that counts has an entry. NaN where nothing counts. last_loss is set as by `loss`."""
         if teacher_tokens.shape[:-1] != tokens.shape:
             raise ValueError(f"teacher_tokens {tuple(teacher_tokens.shape)} must be (..., K) with the tokens' shape "
                              f"{tuple(tokens.shape)}")
@@ -417,7 +417,8 @@ class UnifiedLM(nn.Module):
         if targets is not None:
             counted = targets != -1
             on = on & counted
-        loss = temperature ** 2 * torch.where(on, out.loss, 0.0).sum() / on.sum()
+        n = on.sum() if targets is None else on.sum().clamp(min=1)
+        loss = temperature ** 2 * torch.where(on, out.loss, 0.0).sum() / n
         if targets is not None:
             loss = weight * loss - (1 - weight) * out.logprob.sum() / counted.sum()
         self.last_loss = loss
