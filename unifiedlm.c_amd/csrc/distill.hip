@@ -126,9 +126,10 @@ __device__ __forceinline__ uint32_t bits_at(const uint32_t *mask, int i) {
     return __builtin_amdgcn_alignbit(mask[i / 32 + 1], mask[i / 32], i % 32);
 }
 
-// KEEP, where the cache holds them all: the logits are read as what will be read again. Forward and backward of 2048 rows
-// of 32000 fp32 with the rest 121 us, and 133 with loads that stream in both; of 993 rows of 31999 fp16 46 and 53; of 1 GB
-// of logits 561 and 551.
+// KEEP, where the cache holds them all: the logits are read as what will be read again. Forward and backward with 32 entries,
+// one batch after another, of 4096 rows of 32000 bf16 (250 MiB) 137 us, and 144 with loads that stream in both; of 2048 rows fp32
+// 125 and 130; of 6400 rows bf16 (390 MiB) 216 and 218, of 8192 (500 MiB) 282 and 280; of 1 GB 561 and 551. A forward alone,
+// which nothing follows, is the slower for it: of 4096 rows bf16 49 us and 44, of 2048 rows fp32 47 and 42.
 //
 // One workgroup of NT threads per row, one pass over it, which bounds it: 8192 rows of 32000 bf16 82 us, 6.4 TB/s; 2048
 // rows of 32000 fp32 with the rest 42 us, 6.2 TB/s. The teacher's entries, the token and their logits are read ahead
@@ -309,9 +310,9 @@ constexpr int kBwdVectors = 3;   // a thread
 
 // One workgroup per (row, tile of three vectors a thread). The tile's entries are found first, while its elements are
 // under way: a bit and a value a column. Vectors without an entry or the token, nearly all, take
-// their elements alike. Forward and backward of 16384 rows of 32000 bf16 with 64 entries 550 us, of 2048 rows fp32 with
-// 32 entries and the rest 121. (Loads streaming: 540 and 129; with one vector a thread 679 and 161, so many workgroups
-// look for their entries, with two 540 and 133, with four 533 and 145.)
+// their elements alike. Forward and backward of 16384 rows of 32000 bf16 with 64 entries, at twice the temperature and with
+// the text's tokens, 548 us; of 2048 rows fp32 with 32 entries, the rest and the text's tokens 129. (With one vector a thread
+// 674 and 159, so many workgroups look for their entries; with two 550 and 138, with four 537 and 132.)
 template <int DT, bool REST, Second S, bool KEEP>
 __global__ __launch_bounds__(kThreads) void bwd_kernel(Args a, Grads g, int tiles) {
     constexpr int V = Elem<DT>::vec, B = Elem<DT>::bytes, U = kBwdVectors, kTile = kThreads * V * U;

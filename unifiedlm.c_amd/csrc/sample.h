@@ -543,7 +543,7 @@ __device__ __forceinline__ u64 last_key(const Row<DT, NT> &row, const Draw &d, c
 // units then adds up what lies above them, per wave, and everything, and holds their entries, among
 // which the border is found. The estimate may be wrong, the entries too many: what the units say is
 // looked at, and nothing is kept of it then. idle: min_p leaves less than top_p would, by more than the estimate may be
-// off. (4096 rows of 32000 bf16 with top_k 1000 and top_p: 529 us, and 703 with an exact search behind top_k.)
+// off. (4096 rows of 32000 bf16 with top_k 1000 and top_p: 532 us, and 703 with an exact search behind top_k.)
 template <int DT, int NT>
 __device__ __forceinline__ u64 last_key_by_estimate(const Row<DT, NT> &row, const Draw &d, const Mass &mass, float m,
                                                     u64 least, Scratch<NT> &sc, bool &idle) {
@@ -814,7 +814,7 @@ __device__ __forceinline__ bool draw_short(const Args &a, long long r, const Row
 
 // One workgroup a row. What is kept comes from one of
 //   - the short way: top_k up to 128 (draw_short);
-//   - the estimate: top_p alone (last_key_by_estimate);
+//   - the estimate: top_p, alone or behind a larger top_k (last_key_by_estimate);
 //   - the exact search, which serves all: larger top_k, and where the others give up (last_key);
 //   - nothing to search for: min_p, or no setting.
 // The kept mass of every wave's run is then known; the run in which the token lies is looked through once more.
